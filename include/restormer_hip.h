@@ -535,6 +535,99 @@ int rst_profile_end(char* json, size_t capacity);
 int rst_peak_copy(const void* src, void* dst, size_t bytes, int32_t read_only, void* stream);
 int rst_peak_mfma(int32_t kind, int32_t blocks, int32_t iters, float* out, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Token sequences (norm_rows.hip, causal_conv.hip, scan.hip): the operators of */
+/* a state-space block -- the norm over token rows, the short causal            */
+/* convolution and the selective scan that the reference's training script      */
+/* builds its network from (model/basicsr/archs/mambairv2_arch.py:384-390,      */
+/* mambair_arch.py:356 of the reference call such a scan).                      */
+/*                                                                           */
+/* `dtype` is the storage type of the activations (x, delta, B, C, z, y, the   */
+/* convolution's state and their gradients); parameters, the scan's state and  */
+/* the parameters' gradients are fp32, and so is all arithmetic.  Nothing is   */
+/* assumed about the activations' alignment beyond that of one value.           */
+/* Gradients are overwritten, not accumulated, and come out with the same bits */
+/* from run to run.                                                            */
+/* ------------------------------------------------------------------------- */
+enum rst_dtype { RST_DTYPE_F32 = 0, RST_DTYPE_BF16 = 1 };
+
+/* Layer norm of contiguous rows, x and y: [rows][C], C <= 8192.  bias == NULL: */
+/* the bias-free norm y = x / sqrt(var + eps) * weight (BiasFree_LayerNorm,     */
+/* model/Restromer.py:28-42); else (x - mean) / sqrt(var + eps) * weight + bias */
+/* (WithBias_LayerNorm, :45-61).                                                */
+int rst_rows_norm_fwd(const void* x, int32_t dtype, const float* weight, const float* bias, void* y,
+                      int64_t rows, int32_t C, float eps, void* stream);
+size_t rst_rows_norm_bwd_workspace_bytes(int64_t rows, int32_t C);
+int rst_rows_norm_bwd(const void* x, int32_t dtype, const float* weight, int32_t with_bias, const void* dy,
+                      void* dx, float* dweight, float* dbias, int64_t rows, int32_t C, float eps,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal depthwise convolution of W = 2..4 taps along the tokens, x and y:    */
+/* [B][D][L], weight [D][W] (weight[d][W-1] meets the token itself), bias [D]   */
+/* or NULL, then silu if `silu`.  state_in / state_out [B][D][W-1] (or NULL):   */
+/* the inputs before the first token (NULL: zeros), and the last W-1 inputs     */
+/* (with those of state_in where L is shorter).                                 */
+int rst_causal_conv1d_fwd(const void* x, int32_t dtype, const float* weight, const float* bias, const void* state_in,
+                          void* y, void* state_out, int32_t B, int32_t D, int64_t L, int32_t W, int32_t silu,
+                          void* stream);
+/* dstate_out, dstate_in, dbias may be NULL. */
+size_t rst_causal_conv1d_bwd_workspace_bytes(int32_t B, int32_t D, int64_t L);
+int rst_causal_conv1d_bwd(const void* x, int32_t dtype, const float* weight, const float* bias, const void* state_in,
+                          const void* dy, const void* dstate_out, void* dx, float* dweight, float* dbias,
+                          void* dstate_in, int32_t B, int32_t D, int64_t L, int32_t W, int32_t silu,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* One token, x and y: [B][D].  state_out may be state_in (updated in place). */
+int rst_causal_conv1d_update(const void* x, int32_t dtype, const void* state_in, void* state_out, const float* weight,
+                             const float* bias, void* y, int32_t B, int32_t D, int32_t W, int32_t silu, void* stream);
+
+/* Selective scan.  x, delta, z, y: [B][D][L]; A: [D][N]; B, C: [B][G][N][L],   */
+/* channel d reads group d / (D / G); D, delta_bias: [D] or NULL; z: or NULL;   */
+/* states [B][D][N].  N <= 32.  With dt = softplus(delta + delta_bias) (without */
+/* softplus if !delta_softplus):                                                */
+/*   h_t = exp(dt A) h_{t-1} + dt x B_t,   y = sum_n C h + D x,  times silu(z)  */
+typedef struct rst_scan_desc {
+    int32_t B, D, G, N;
+    int64_t L;
+    int32_t dtype;
+    int32_t delta_softplus;
+} rst_scan_desc;
+typedef struct rst_scan_inputs {
+    const void*  x;
+    const void*  delta;
+    const float* A;
+    const void*  B;
+    const void*  C;
+    const float* D;
+    const void*  z;
+    const float* delta_bias;
+} rst_scan_inputs;
+/* D, delta_bias: or NULL where their gradient is not wanted; z: with inputs->z. */
+typedef struct rst_scan_grads {
+    void*  x;
+    void*  delta;
+    float* A;
+    void*  B;
+    void*  C;
+    float* D;
+    void*  z;
+    float* delta_bias;
+} rst_scan_grads;
+/* state_in, state_out: or NULL.  saved: rst_scan_saved_bytes for a backward    */
+/* pass (the states every 16 tokens), or NULL.  Workspaces aligned to 16 bytes. */
+size_t rst_scan_workspace_bytes(const rst_scan_desc* desc);
+size_t rst_scan_saved_bytes(const rst_scan_desc* desc);
+int rst_scan_fwd(const rst_scan_desc* desc, const rst_scan_inputs* inputs, const float* state_in, void* y,
+                 float* state_out, float* saved, void* workspace, size_t workspace_bytes, void* stream);
+/* dstate_out, dstate_in: or NULL. */
+size_t rst_scan_bwd_workspace_bytes(const rst_scan_desc* desc);
+int rst_scan_bwd(const rst_scan_desc* desc, const rst_scan_inputs* inputs, const float* saved, const void* dy,
+                 const float* dstate_out, const rst_scan_grads* grads, float* dstate_in,
+                 void* workspace, size_t workspace_bytes, void* stream);
+/* One token (desc->L = 1; x, delta, z, y: [B][D]; B, C: [B][G][N]).  state_out */
+/* may be state_in.                                                             */
+int rst_scan_update(const rst_scan_desc* desc, const rst_scan_inputs* inputs, const float* state_in, float* state_out,
+                    void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

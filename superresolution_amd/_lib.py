@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # (RST_LIB_PATH: another build of the same library, for A/B timing of kernel variants)
@@ -38,10 +38,30 @@ class BlockGrads(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in PARAM_FIELDS]
 
 
+class ScanDesc(ctypes.Structure):
+    """rst_scan_desc"""
+    _fields_ = [("B", c_int32), ("D", c_int32), ("G", c_int32), ("N", c_int32), ("L", c_int64), ("dtype", c_int32),
+                ("delta_softplus", c_int32)]
+
+
+SCAN_FIELDS = ("x", "delta", "A", "B", "C", "D", "z", "delta_bias")
+
+
+class ScanInputs(ctypes.Structure):
+    """rst_scan_inputs"""
+    _fields_ = [(n, c_void_p) for n in SCAN_FIELDS]
+
+
+class ScanGrads(ctypes.Structure):
+    """rst_scan_grads"""
+    _fields_ = [(n, c_void_p) for n in SCAN_FIELDS]
+
+
 _P = c_void_p
 _DESC = POINTER(BlockDesc)
 _PAR = POINTER(BlockParams)
 _GR = POINTER(BlockGrads)
+_SD, _SI, _SG = POINTER(ScanDesc), POINTER(ScanInputs), POINTER(ScanGrads)
 
 # name -> (restype, argtypes); every symbol declared in include/restormer_hip.h
 SIGNATURES = {
@@ -125,6 +145,20 @@ SIGNATURES = {
     "rst_conv3x3_bwd_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "rst_conv3x3_bwd": (c_int32, [_P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _P, c_size_t, _P]),
     "rst_raw_prepare": (c_int32, [_P, c_int32, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, _P]),
+    "rst_rows_norm_fwd": (c_int32, [_P, c_int32, _P, _P, _P, c_int64, c_int32, c_float, _P]),
+    "rst_rows_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int32]),
+    "rst_rows_norm_bwd": (c_int32, [_P, c_int32, _P, c_int32, _P, _P, _P, _P, c_int64, c_int32, c_float, _P, c_size_t, _P]),
+    "rst_causal_conv1d_fwd": (c_int32, [_P, c_int32, _P, _P, _P, _P, _P, c_int32, c_int32, c_int64, c_int32, c_int32, _P]),
+    "rst_causal_conv1d_bwd_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int64]),
+    "rst_causal_conv1d_bwd": (c_int32, [_P, c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int64, c_int32, c_int32,
+                                        _P, c_size_t, _P]),
+    "rst_causal_conv1d_update": (c_int32, [_P, c_int32, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, _P]),
+    "rst_scan_workspace_bytes": (c_size_t, [_SD]),
+    "rst_scan_saved_bytes": (c_size_t, [_SD]),
+    "rst_scan_fwd": (c_int32, [_SD, _SI, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "rst_scan_bwd_workspace_bytes": (c_size_t, [_SD]),
+    "rst_scan_bwd": (c_int32, [_SD, _SI, _P, _P, _P, _SG, _P, _P, c_size_t, _P]),
+    "rst_scan_update": (c_int32, [_SD, _SI, _P, _P, _P, _P]),
     "rst_profile_begin": (c_int32, []),
     "rst_profile_end": (c_int32, [c_char_p, c_size_t]),
     "rst_peak_copy": (c_int32, [_P, _P, c_size_t, c_int32, _P]),

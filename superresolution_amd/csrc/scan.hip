@@ -1,0 +1,803 @@
+// Selective state space scan over the tokens of every channel (x, delta, z, y: [B][D][L]; A: [D][N]; B, C: [B][G][N][L],
+// channel d reads group d / (D/G)), its backward pass, and its form for one token.
+//
+//   dt = softplus(delta + bias),  a_t[n] = exp(dt_t A[n]),  h_t[n] = a_t[n] h_{t-1}[n] + dt_t x_t B_t[n]
+//   s_t = sum_n C_t[n] h_t[n] + D x_t,   y_t = s_t or s_t silu(z_t)
+//   backward, e_t = dy_t silu(z_t):  g_t[n] = C_t[n] e_t + a_{t+1}[n] g_{t+1}[n]   (from the last token to the first)
+//   dC_t[n] = sum_d h e,  dB_t[n] = sum_d g dt x,  dx = dt sum_n g B + D e,  ddt = x sum_n g B + sum_n A a g h_{t-1},
+//   dA[n] = sum_{b,t} dt a g h_{t-1},  dD = sum e x,  ddelta = ddt sigmoid(delta + bias),  dz = dy s silu'(z)
+//
+// Bound by the vector pipe, not by memory: one exponential and five more operations per state and token forward (16
+// states: 96 operations for the 6 to 12 bytes of a bf16 or fp32 token), so the layout serves the instruction stream:
+//   - a lane is a channel and holds four of its states; the waves of a block hold the other states of the same 64
+//     channels.  B and C are then the same for a whole wave and come in as scalar operands (no vector register, no LDS).
+//     They are laid out for that once per call: [B][G][token][wave][B0..B3 C0..C3] in fp32 (bc_prep_kernel).
+//   - tokens go in tiles of 16.  The tensors are token-contiguous, so a thread loads 4 tokens of one channel (a wave: 16
+//     channels x 16 tokens), takes softplus once, and hands dt and dt x over through LDS, turned to lane = channel; the
+//     waves' shares of s come back the same way.
+//   - where there are too few channels to fill the chip, the tokens are cut into chunks: a first kernel takes every
+//     chunk's own end state and the sum of its dt (its decay is exp(A sum dt)), and a chunk starts from the combination
+//     of those before it.  That costs the exponentials a second time, so it is done only then (scan_plan).
+//   - backward, a wave forms the tile's 16 x 4 states again from the state at the tile's start (kept by the forward
+//     pass), holds them and the decays in registers, and walks back.
+// State, decay, sums and partial sums are fp32.
+#include "seq_common.hpp"
+
+namespace rst {
+
+constexpr int ST = 16;                 // tokens of a tile
+constexpr int SC = 64;                 // channels of a block
+constexpr int SROW = 68;               // LDS row of a token: 64 channels, padded so that 4 tokens apart is 16 banks apart
+
+struct Scan {
+    const void *x, *delta, *Bm, *Cm, *z, *dy;
+    const float *A, *Dskip, *dbias, *h0, *dlast;
+    void *y, *dx, *ddelta, *dB, *dC, *dz;
+    float *last, *dh0;
+    float* bc;                          // [B][G][tiles * 16][W][8]
+    float* ckpt;                        // [B][tiles][4 W][D]: the state at every tile's start, or null
+    float* cst;                         // [B][chunks][4 W][D]: what a chunk adds to the state behind (backward: before) it
+    float* cdt;                         // [B][chunks][D]: sum of dt
+    float* bcpart;                      // [channel blocks of a group][B][G][tiles * 16][W][8]: shares of dB and dC
+    float* dApart;                      // [B][chunks][4 W][D]
+    float* dDpart;                      // [B][chunks][2][D]: dD, dbias
+    int B, D, G, N, Dg, cb;             // cb: channel blocks of a group
+    int64_t L;
+    int tiles, nchunk, per_chunk;       // per_chunk: tiles
+    int softplus;
+};
+
+// log(1 + e^v): 1 + e^v loses the low bits of a small e^v, and log(w) e / (w - 1) gives them back
+__device__ __forceinline__ float softplus(float v) {
+    if (v > 20.f) return v;
+    const float e = exp_near(v), w = 1.0f + e;
+    const float l = __builtin_amdgcn_logf(w) * 0.6931471805599453f;
+    return w == 1.0f ? e : l * e * rcp_fast(w - 1.0f);
+}
+
+// which chunk, sample, group and channels a block has
+struct ScanPlace {
+    int b, g, cb, chunk, lane, wave;
+    __device__ __forceinline__ ScanPlace(const Scan& a, int chunks, int first) {
+        const uint32_t per = (uint32_t)(a.G * a.cb);
+        uint32_t i = blockIdx.x;
+        const uint32_t gc = i % per;
+        i /= per;
+        chunk = (int)(i % (uint32_t)chunks) + first;
+        b = (int)(i / (uint32_t)chunks);
+        g = (int)gc / a.cb;
+        cb = (int)gc % a.cb;
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    }
+};
+
+// four tokens of one channel
+template <typename T> struct Quad {
+    Raw<T, 4> r;
+    __device__ __forceinline__ void load(const T* row, int64_t t, int64_t L, bool ok) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(r.w) / 4); ++i) r.w[i] = 0;
+        if (!ok) return;
+        if (t + 4 <= L) { r.load(row + t); return; }
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = t + i < L ? Store<T>::get(row[t + i]) : 0.f;
+        r.pack(v);
+    }
+    static __device__ __forceinline__ void put(T* row, int64_t t, int64_t L, bool ok, const float (&v)[4]) {
+        if (!ok) return;
+        if (t + 4 <= L) {
+            Raw<T, 4> o;
+            o.pack(v);
+            o.store(row + t);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (t + i < L) row[t + i] = Store<T>::put(v[i]);
+    }
+};
+
+// a block of W waves has 64 channels x 4 quads of a tile to load: items per thread
+template <int W> struct ScanItems { static constexpr int N = W >= 4 ? 1 : 4 / W; };
+
+// the channel, quad and address of one of a thread's items
+template <int W> struct ScanItem {
+    int r, q, d; bool ok; int64_t row;
+    __device__ __forceinline__ ScanItem() {}
+    __device__ __forceinline__ void set(const Scan& a, const ScanPlace& p, int k) {
+        const int i = threadIdx.x + k * 64 * W;
+        r = (i >> 2) & 63;
+        q = i & 3;
+        d = p.g * a.Dg + p.cb * SC + r;
+        ok = i < 256 && p.cb * SC + r < a.Dg;
+        row = ((int64_t)p.b * a.D + (ok ? d : 0)) * a.L;
+    }
+    static __device__ __forceinline__ bool has(int k) { return threadIdx.x + k * 64 * W < 256; }
+};
+
+__device__ __forceinline__ float step_size(const Scan& a, float raw) { return a.softplus ? softplus(raw) : raw; }
+
+// B and C as the scan's waves read them: [b][g][token][wave][B0..B3 C0..C3], zeros behind the last state and token.
+// Threads run along the tokens, so the reads are whole lines.
+template <typename T>
+__global__ void __launch_bounds__(256)
+bc_prep_kernel(const T* __restrict__ Bm, const T* __restrict__ Cm, float* __restrict__ bc, int N, int W, int64_t L, int64_t Lp) {
+    const int64_t t = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int64_t bg = blockIdx.y;
+    if (t >= Lp) return;
+    for (int w = threadIdx.x >> 6; w < W; w += 4) {
+        float v[8];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int n = w * 4 + s;
+            const bool in = n < N && t < L;
+            v[s] = in ? Store<T>::get(Bm[(bg * N + n) * L + t]) : 0.f;
+            v[4 + s] = in ? Store<T>::get(Cm[(bg * N + n) * L + t]) : 0.f;
+        }
+        Raw<float, 8> o;
+        o.pack(v);
+        o.store(bc + ((bg * Lp + t) * W + w) * 8);
+    }
+}
+
+// A (times log2 e) of the lane's channel and four states; zero where there are none, so that they stay zero
+__device__ __forceinline__ void load_rates(const Scan& a, int d, bool ok, int wave, float (&A)[4]) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) A[s] = ok && wave * 4 + s < a.N ? a.A[(int64_t)d * a.N + wave * 4 + s] : 0.f;
+}
+
+// ---- what a chunk adds to the state behind it (REV: to the state's gradient before it), and the sum of its dt -------
+template <typename T, int W, bool REV>
+__global__ void __launch_bounds__(64 * W)
+scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
+    constexpr int NI = ScanItems<W>::N;
+    __shared__ float dts[ST][SROW], us[ST][SROW];
+    const ScanPlace p(a, a.nchunk - 1, REV ? 1 : 0);
+    const int d = p.g * a.Dg + p.cb * SC + p.lane;
+    const bool ok = p.cb * SC + p.lane < a.Dg;
+    float A[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+    load_rates(a, d, ok, p.wave, A);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) A[s] *= LOG2E;
+    const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
+    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave) * 8;
+    ScanItem<W> it[NI];
+    float bias[NI];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+        it[k].set(a, p, k);
+        bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
+    }
+    for (int n = 0; n < t1 - t0; ++n) {
+        const int tile = REV ? t1 - 1 - n : t0 + n;
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
+            Quad<T> qd, qx, qz;
+            qd.load(static_cast<const T*>(a.delta) + it[k].row, t, a.L, it[k].ok);
+            qx.load(static_cast<const T*>(REV ? a.dy : a.x) + it[k].row, t, a.L, it[k].ok);
+            if (REV && a.z) qz.load(static_cast<const T*>(a.z) + it[k].row, t, a.L, it[k].ok);
+            if (ScanItem<W>::has(k)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float dt = it[k].ok && t + i < a.L ? step_size(a, qd.r.get(i) + bias[k]) : 0.f;
+                    float u;
+                    if (REV) {
+                        u = qx.r.get(i);
+                        if (a.z) { const float z = qz.r.get(i); u *= z * sigmoid(z); }
+                    } else u = dt * qx.r.get(i);
+                    dts[it[k].q * 4 + i][it[k].r] = dt;
+                    us[it[k].q * 4 + i][it[k].r] = u;
+                }
+            }
+        }
+        __syncthreads();
+        const float* bt = bc + (int64_t)tile * ST * W * 8;
+#pragma unroll 4
+        for (int i = 0; i < ST; ++i) {
+            const int tt = REV ? ST - 1 - i : i;
+            const float* v = bt + tt * W * 8;
+            const float dt = dts[tt][p.lane], u = us[tt][p.lane];
+            sum += dt;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float decay = __builtin_amdgcn_exp2f(dt * A[s]);
+                if (REV) h[s] = decay * fmaf(u, v[4 + s], h[s]);
+                else h[s] = fmaf(decay, h[s], u * v[s]);
+            }
+        }
+        __syncthreads();
+    }
+    if (ok) {
+        const int64_t c = (int64_t)p.b * a.nchunk + p.chunk;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a.cst[(c * 4 * W + p.wave * 4 + s) * a.D + d] = h[s];
+        if (p.wave == 0) a.cdt[c * a.D + d] = sum;
+    }
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+template <typename T, int W>
+__global__ void __launch_bounds__(64 * W)
+scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
+    constexpr int NI = ScanItems<W>::N;
+    __shared__ float dts[ST][SROW], us[ST][SROW], part[W][ST][SROW];
+    const ScanPlace p(a, a.nchunk, 0);
+    const int d = p.g * a.Dg + p.cb * SC + p.lane;
+    const bool ok = p.cb * SC + p.lane < a.Dg;
+    float A[4], h[4];
+    load_rates(a, d, ok, p.wave, A);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        A[s] *= LOG2E;
+        h[s] = a.h0 && ok && p.wave * 4 + s < a.N ? a.h0[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
+    }
+    for (int c = 0; c < p.chunk; ++c) {
+        const int64_t ci = (int64_t)p.b * a.nchunk + c;
+        const float sum = ok ? a.cdt[ci * a.D + d] : 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            h[s] = fmaf(__builtin_amdgcn_exp2f(sum * A[s]), h[s], ok ? a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + d] : 0.f);
+    }
+    const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
+    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave) * 8;
+    ScanItem<W> it[NI];
+    float bias[NI], skip[NI];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+        it[k].set(a, p, k);
+        bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
+        skip[k] = a.Dskip && it[k].ok ? a.Dskip[it[k].d] : 0.f;
+    }
+    for (int tile = t0; tile < t1; ++tile) {
+        float x[NI][4];
+        Quad<T> qz[NI];
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
+            Quad<T> qd, qx;
+            qd.load(static_cast<const T*>(a.delta) + it[k].row, t, a.L, it[k].ok);
+            qx.load(static_cast<const T*>(a.x) + it[k].row, t, a.L, it[k].ok);
+            if (a.z) qz[k].load(static_cast<const T*>(a.z) + it[k].row, t, a.L, it[k].ok);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float dt = it[k].ok && t + i < a.L ? step_size(a, qd.r.get(i) + bias[k]) : 0.f;
+                x[k][i] = qx.r.get(i);
+                if (ScanItem<W>::has(k)) {
+                    dts[it[k].q * 4 + i][it[k].r] = dt;
+                    us[it[k].q * 4 + i][it[k].r] = dt * x[k][i];
+                }
+            }
+        }
+        __syncthreads();
+        if (a.ckpt && ok) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + d] = h[s];
+        }
+        const float* bt = bc + (int64_t)tile * ST * W * 8;
+#pragma unroll 4
+        for (int i = 0; i < ST; ++i) {
+            const float* v = bt + i * W * 8;
+            const float dt = dts[i][p.lane], u = us[i][p.lane];
+            float y = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                h[s] = fmaf(__builtin_amdgcn_exp2f(dt * A[s]), h[s], u * v[s]);
+                y = fmaf(v[4 + s], h[s], y);
+            }
+            part[p.wave][i][p.lane] = y;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            if (!ScanItem<W>::has(k)) continue;
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float s = skip[k] * x[k][i];
+#pragma unroll
+                for (int w = 0; w < W; ++w) s += part[w][it[k].q * 4 + i][it[k].r];
+                if (a.z) { const float z = qz[k].r.get(i); s *= z * sigmoid(z); }
+                y[i] = s;
+            }
+            Quad<T>::put(static_cast<T*>(a.y) + it[k].row, (int64_t)tile * ST + it[k].q * 4, a.L, it[k].ok, y);
+        }
+    }
+    if (a.last && ok && t1 == a.tiles) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (p.wave * 4 + s < a.N) a.last[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] = h[s];
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------
+template <typename T, int W>
+__global__ void __launch_bounds__(64 * W)
+scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
+    constexpr int NI = ScanItems<W>::N;
+    extern __shared__ __attribute__((aligned(16))) float smem[];
+    float (*dts)[SROW] = reinterpret_cast<float (*)[SROW]>(smem);
+    float (*us)[SROW] = dts + ST;
+    float (*es)[SROW] = us + ST;
+    float (*part0)[ST][SROW] = reinterpret_cast<float (*)[ST][SROW]>(es + ST);          // [W]: shares of s, then of sum g B
+    float (*part1)[ST][SROW] = part0 + W;                                               // [W]: shares of sum A a g h
+    const ScanPlace p(a, a.nchunk, 0);
+    const int d = p.g * a.Dg + p.cb * SC + p.lane;
+    const bool ok = p.cb * SC + p.lane < a.Dg;
+    float A[4], A2[4], g[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
+    load_rates(a, d, ok, p.wave, A);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        A2[s] = A[s] * LOG2E;
+        g[s] = a.dlast && ok && p.wave * 4 + s < a.N ? a.dlast[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
+    }
+    for (int c = a.nchunk - 1; c > p.chunk; --c) {
+        const int64_t ci = (int64_t)p.b * a.nchunk + c;
+        const float sum = ok ? a.cdt[ci * a.D + d] : 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            g[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), g[s], ok ? a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + d] : 0.f);
+    }
+    const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
+    const int64_t bg = (int64_t)p.b * a.G + p.g;
+    const float* bc = bc0 + (bg * a.tiles * ST * W + p.wave) * 8;
+    float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * ST * W + p.wave) * 8;
+    ScanItem<W> it[NI];
+    float bias[NI], skip[NI], dD[NI], db[NI];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+        it[k].set(a, p, k);
+        bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
+        skip[k] = a.Dskip && it[k].ok ? a.Dskip[it[k].d] : 0.f;
+        dD[k] = 0.f;
+        db[k] = 0.f;
+    }
+    for (int tile = t1 - 1; tile >= t0; --tile) {
+        float x[NI][4], dt[NI][4], e[NI][4], raw[NI][4];
+        Quad<T> qz[NI], qy[NI];
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
+            Quad<T> qd, qx;
+            qd.load(static_cast<const T*>(a.delta) + it[k].row, t, a.L, it[k].ok);
+            qx.load(static_cast<const T*>(a.x) + it[k].row, t, a.L, it[k].ok);
+            qy[k].load(static_cast<const T*>(a.dy) + it[k].row, t, a.L, it[k].ok);
+            if (a.z) qz[k].load(static_cast<const T*>(a.z) + it[k].row, t, a.L, it[k].ok);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                raw[k][i] = qd.r.get(i) + bias[k];
+                dt[k][i] = it[k].ok && t + i < a.L ? step_size(a, raw[k][i]) : 0.f;
+                x[k][i] = qx.r.get(i);
+                e[k][i] = qy[k].r.get(i);
+                if (a.z) { const float z = qz[k].r.get(i); e[k][i] *= z * sigmoid(z); }
+                if (ScanItem<W>::has(k)) {
+                    dts[it[k].q * 4 + i][it[k].r] = dt[k][i];
+                    us[it[k].q * 4 + i][it[k].r] = dt[k][i] * x[k][i];
+                    es[it[k].q * 4 + i][it[k].r] = e[k][i];
+                }
+            }
+        }
+        float hs[ST + 1][4], as[ST][4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            hs[0][s] = ok ? a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + d] : 0.f;
+        __syncthreads();
+        const float* bt = bc + (int64_t)tile * ST * W * 8;
+#pragma unroll
+        for (int i = 0; i < ST; ++i) {
+            const float* v = bt + i * W * 8;
+            const float dti = dts[i][p.lane], u = us[i][p.lane];
+            float y = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                as[i][s] = __builtin_amdgcn_exp2f(dti * A2[s]);
+                hs[i + 1][s] = fmaf(as[i][s], hs[i][s], u * v[s]);
+                if (a.z) y = fmaf(v[4 + s], hs[i + 1][s], y);
+            }
+            if (a.z) part0[p.wave][i][p.lane] = y;
+        }
+        float dz[NI][4];
+        if (a.z) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < NI; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!ScanItem<W>::has(k)) continue;
+                    float s = skip[k] * x[k][i];
+#pragma unroll
+                    for (int w = 0; w < W; ++w) s += part0[w][it[k].q * 4 + i][it[k].r];
+                    const float z = qz[k].r.get(i), q = sigmoid(z);
+                    dz[k][i] = qy[k].r.get(i) * s * (q * fmaf(z, 1.0f - q, 1.0f));
+                }
+            __syncthreads();
+        }
+        float tA[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = ST - 1; i >= 0; --i) {
+            const float* v = bt + i * W * 8;
+            const float dti = dts[i][p.lane], u = us[i][p.lane], ei = es[i][p.lane];
+            float gB = 0.f, gA = 0.f, pr[8];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                g[s] = fmaf(v[4 + s], ei, g[s]);
+                pr[s] = g[s] * u;
+                pr[4 + s] = hs[i + 1][s] * ei;
+                gB = fmaf(g[s], v[s], gB);
+                g[s] *= as[i][s];
+                const float q = g[s] * hs[i][s];
+                gA = fmaf(A[s], q, gA);
+                tA[s] = fmaf(dti, q, tA[s]);
+            }
+            part0[p.wave][i][p.lane] = gB;
+            part1[p.wave][i][p.lane] = gA;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const float v8 = wave_sum(ok ? pr[s] : 0.f);       // (no channel there: 0 times an infinite C is no zero)
+                if (p.lane == s) bco[((int64_t)tile * ST + i) * W * 8 + s] = v8;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) dA[s] += tA[s];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            if (!ScanItem<W>::has(k)) continue;
+            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
+            float ox[4], od[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float gB = 0.f, gA = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    gB += part0[w][it[k].q * 4 + i][it[k].r];
+                    gA += part1[w][it[k].q * 4 + i][it[k].r];
+                }
+                ox[i] = fmaf(gB, dt[k][i], skip[k] * e[k][i]);
+                od[i] = fmaf(gB, x[k][i], gA);
+                if (a.softplus) od[i] *= sigmoid(raw[k][i]);
+                if (it[k].ok && t + i < a.L) {
+                    dD[k] = fmaf(e[k][i], x[k][i], dD[k]);
+                    db[k] += od[i];
+                }
+            }
+            Quad<T>::put(static_cast<T*>(a.dx) + it[k].row, t, a.L, it[k].ok, ox);
+            Quad<T>::put(static_cast<T*>(a.ddelta) + it[k].row, t, a.L, it[k].ok, od);
+            if (a.z) Quad<T>::put(static_cast<T*>(a.dz) + it[k].row, t, a.L, it[k].ok, dz[k]);
+        }
+        __syncthreads();
+    }
+    const int64_t c = (int64_t)p.b * a.nchunk + p.chunk;
+    if (ok) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            a.dApart[(c * 4 * W + p.wave * 4 + s) * a.D + d] = dA[s];
+            if (a.dh0 && p.chunk == 0 && p.wave * 4 + s < a.N) a.dh0[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] = g[s];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+            dD[k] += __shfl_xor(dD[k], off, 64);
+            db[k] += __shfl_xor(db[k], off, 64);
+        }
+        if (it[k].ok && it[k].q == 0) {
+            a.dDpart[(c * 2 + 0) * a.D + it[k].d] = dD[k];
+            a.dDpart[(c * 2 + 1) * a.D + it[k].d] = db[k];
+        }
+    }
+}
+
+// dB, dC [B][G][N][L]: the channel blocks' shares in a fixed order, turned back to token-contiguous
+template <typename T>
+__global__ void __launch_bounds__(256)
+scan_reduce_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC, int cb, int64_t stride, int N, int W,
+                      int64_t L, int64_t Lp) {
+    const int64_t t = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int64_t bg = blockIdx.y;
+    if (t >= L) return;
+    for (int w = threadIdx.x >> 6; w < W; w += 4) {
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < cb; ++c) {
+            Raw<float, 8> v;
+            v.load(part + c * stride + ((bg * Lp + t) * W + w) * 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += v.get(i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = w * 4 + i;
+            if (n < N) {
+                dB[(bg * N + n) * L + t] = Store<T>::put(s[i]);
+                dC[(bg * N + n) * L + t] = Store<T>::put(s[4 + i]);
+            }
+        }
+    }
+}
+
+// dA [D][N], dD [D], dbias [D]: the shares of all samples and chunks in a fixed order.  Rows 0 .. N-1 are dA's states,
+// N is dD, N + 1 dbias; lanes run along the channels.
+__global__ void __launch_bounds__(256)
+scan_reduce_params_kernel(const float* __restrict__ dApart, const float* __restrict__ dDpart, float* __restrict__ dA,
+                          float* __restrict__ dD, float* __restrict__ dbias, int n, int D, int N, int W) {
+    __shared__ float red[16][17];
+    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
+    const int d = blockIdx.x * 16 + col, row = blockIdx.y;
+    float s = 0.f;
+    if (d < D)
+        for (int64_t c = slice; c < n; c += 16)
+            s += row < N ? dApart[(c * 4 * W + row) * D + d] : dDpart[(c * 2 + row - N) * D + d];
+    red[slice][col] = s;
+    __syncthreads();
+    for (int h = 8; h > 0; h >>= 1) {
+        if (slice < h) red[slice][col] += red[slice + h][col];
+        __syncthreads();
+    }
+    if (slice != 0 || d >= D) return;
+    if (row < N) dA[(int64_t)d * N + row] = red[0][col];
+    else if (row == N) { if (dD) dD[d] = red[0][col]; }
+    else if (dbias) dbias[d] = red[0][col];
+}
+
+// ---- one token -----------------------------------------------------------------------------------------------------
+// NL lanes share a channel, four states each.  Bound by the state's 8 N bytes per channel.  state_out may be the state.
+template <typename T, int NL>
+__global__ void __launch_bounds__(256)
+scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const float* __restrict__ A, const T* __restrict__ Bm,
+                   const T* __restrict__ Cm, const float* __restrict__ Dskip, const T* __restrict__ z,
+                   const float* __restrict__ dbias, const float* state, float* state_out, T* __restrict__ y, int64_t n, int D, int G,
+                   int N, int soft) {
+    const int64_t i = (int64_t)blockIdx.x * (256 / NL) + threadIdx.x / NL;
+    const int lane = threadIdx.x % NL;
+    const bool live = i < n;
+    float s = 0.f, xv = 0.f;
+    if (live) {
+        const int d = (int)((uint32_t)i % (uint32_t)D), b = (int)((uint32_t)i / (uint32_t)D);
+        const int64_t bg = (int64_t)b * G + d / (D / G);
+        xv = Store<T>::get(x[i]);
+        float dt = Store<T>::get(delta[i]) + (dbias ? dbias[d] : 0.f);
+        if (soft) dt = softplus(dt);
+        const float u = dt * xv;
+        float h[4], Av[4];
+        const int n0 = lane * 4;
+        if ((N & 3) == 0 && n0 < N) {
+            Raw<float, 4> hv, av;
+            hv.load(state + i * N + n0);
+            av.load(A + (int64_t)d * N + n0);
+            hv.unpack(h);
+            av.unpack(Av);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h[k] = n0 + k < N ? state[i * N + n0 + k] : 0.f;
+                Av[k] = n0 + k < N ? A[(int64_t)d * N + n0 + k] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n0 + k < N) {
+                h[k] = fmaf(exp_fast(dt * Av[k]), h[k], u * Store<T>::get(Bm[bg * N + n0 + k]));
+                s = fmaf(Store<T>::get(Cm[bg * N + n0 + k]), h[k], s);
+            }
+        if ((N & 3) == 0 && n0 < N) {
+            Raw<float, 4> hv;
+            hv.pack(h);
+            hv.store(state_out + i * N + n0);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (n0 + k < N) state_out[i * N + n0 + k] = h[k];
+        }
+        if (lane == 0 && Dskip) s = fmaf(Dskip[d], xv, s);
+    }
+#pragma unroll
+    for (int off = NL / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (live && lane == 0) {
+        if (z) { const float zv = Store<T>::get(z[i]); s *= zv * sigmoid(zv); }
+        y[i] = Store<T>::put(s);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
+
+// Chunks: enough blocks for two of them on each of the 256 compute units, chunks of at least four tiles.
+static void scan_plan(Scan* a) {
+    a->Dg = a->D / a->G;
+    a->cb = (int)cdiv(a->Dg, SC);
+    a->tiles = (int)cdiv(a->L, ST);
+    const int64_t blocks = (int64_t)a->B * a->G * a->cb;
+    int64_t want = cdiv(512, blocks);
+    const int64_t most = a->tiles / 4 > 1 ? a->tiles / 4 : 1;
+    if (want > most) want = most;
+    a->per_chunk = (int)cdiv(a->tiles, want);
+    a->nchunk = (int)cdiv(a->tiles, a->per_chunk);
+}
+
+static int scan_check(const char* what, const rst_scan_desc* s) {
+    RST_REQUIRE(s != nullptr, "%s: null descriptor", what);
+    RST_REQUIRE(s->dtype == RST_DTYPE_F32 || s->dtype == RST_DTYPE_BF16, "%s: unknown dtype %d", what, s->dtype);
+    RST_REQUIRE(s->B > 0 && s->D > 0 && s->L > 0, "%s: empty shape B=%d D=%d L=%lld", what, s->B, s->D, (long long)s->L);
+    RST_REQUIRE(s->G > 0 && s->D % s->G == 0, "%s: D=%d not divisible by groups=%d", what, s->D, s->G);
+    RST_REQUIRE(s->N > 0 && s->N <= 32, "%s: N=%d states (1 to 32)", what, s->N);
+    RST_REQUIRE(s->L <= (1ll << 31) && (int64_t)s->B * s->D <= (1ll << 30) && (int64_t)s->B * s->G <= 65535,
+                "%s: shape out of range B=%d D=%d G=%d L=%lld", what, s->B, s->D, s->G, (long long)s->L);
+    return RST_OK;
+}
+
+static void scan_shape(Scan* a, const rst_scan_desc* s) {
+    a->B = s->B; a->D = s->D; a->G = s->G; a->N = s->N; a->L = s->L; a->softplus = s->delta_softplus;
+    scan_plan(a);
+}
+
+// Scratch of a call, carved from the caller's workspace (base == null: only measured)
+static size_t scan_carve(Scan* a, char* base, bool bwd) {
+    const int W = scan_waves(a->N);
+    size_t off = 0;
+    auto take = [&](int64_t floats) {
+        float* p = base ? reinterpret_cast<float*>(base + off) : nullptr;
+        off = (off + (size_t)floats * sizeof(float) + 255) & ~size_t(255);
+        return p;
+    };
+    const int64_t bcf = (int64_t)a->B * a->G * a->tiles * ST * W * 8, chunks = (int64_t)a->B * a->nchunk;
+    a->bc = take(bcf);
+    if (a->nchunk > 1) {
+        a->cst = take(chunks * 4 * W * a->D);
+        a->cdt = take(chunks * a->D);
+    }
+    if (bwd) {
+        a->bcpart = take(bcf * a->cb);
+        a->dApart = take(chunks * 4 * W * a->D);
+        a->dDpart = take(chunks * 2 * a->D);
+    }
+    return off;
+}
+
+template <typename T>
+static int scan_prep(const Scan& a, int W, hipStream_t st) {
+    const int64_t Lp = (int64_t)a.tiles * ST;
+    hipLaunchKernelGGL((bc_prep_kernel<T>), dim3((unsigned)cdiv(Lp, 64), a.B * a.G), dim3(256), 0, st, static_cast<const T*>(a.Bm),
+                       static_cast<const T*>(a.Cm), a.bc, a.N, W, a.L, Lp);
+    RST_LAUNCH_CHECK();
+    return RST_OK;
+}
+
+template <typename T, int W>
+static int scan_fwd_t(const Scan& a, hipStream_t st) {
+    const double n = (double)a.B * a.D * a.L;
+    ProfScope prof(st, "scan_fwd", n * (7.0 * a.N + 12), sizeof(T) * n * (a.z ? 4 : 3));
+    RST_TRY(scan_prep<T>(a, W, st));
+    const int64_t per = (int64_t)a.B * a.G * a.cb;
+    RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
+    if (a.nchunk > 1) {
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        RST_LAUNCH_CHECK();
+    }
+    hipLaunchKernelGGL((scan_fwd_kernel<T, W>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a, a.bc);
+    RST_LAUNCH_CHECK();
+    return RST_OK;
+}
+
+template <typename T, int W>
+static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStream_t st) {
+    const double n = (double)a.B * a.D * a.L;
+    ProfScope prof(st, "scan_bwd", n * (16.0 * a.N + 28), sizeof(T) * n * (a.z ? 7 : 5));
+    RST_TRY(scan_prep<T>(a, W, st));
+    const int64_t per = (int64_t)a.B * a.G * a.cb;
+    RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
+    if (a.nchunk > 1) {
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        RST_LAUNCH_CHECK();
+    }
+    const size_t lds = (size_t)(3 + 2 * W) * ST * SROW * sizeof(float);
+    KernelSetup ks;
+    RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W>), 64 * W, lds, &ks));
+    hipLaunchKernelGGL((scan_bwd_kernel<T, W>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a, a.bc);
+    RST_LAUNCH_CHECK();
+    const int64_t Lp = (int64_t)a.tiles * ST;
+    hipLaunchKernelGGL((scan_reduce_bc_kernel<T>), dim3((unsigned)cdiv(a.L, 64), a.B * a.G), dim3(256), 0, st, a.bcpart,
+                       static_cast<T*>(a.dB), static_cast<T*>(a.dC), a.cb, (int64_t)a.B * a.G * Lp * W * 8, a.N, W, a.L, Lp);
+    RST_LAUNCH_CHECK();
+    hipLaunchKernelGGL(scan_reduce_params_kernel, dim3((unsigned)cdiv(a.D, 16), a.N + 2), dim3(256), 0, st, a.dApart, a.dDpart, dA, dD,
+                       dbias, a.B * a.nchunk, a.D, a.N, W);
+    RST_LAUNCH_CHECK();
+    return RST_OK;
+}
+
+template <typename T, int NL>
+static int scan_update_t(const rst_scan_desc* s, const rst_scan_inputs* in, const float* state, float* state_out, T* y, hipStream_t st) {
+    const int64_t n = (int64_t)s->B * s->D;
+    ProfScope prof(st, "scan_update", n * (7.0 * s->N + 20), n * 8.0 * s->N);
+    hipLaunchKernelGGL((scan_update_kernel<T, NL>), dim3((unsigned)cdiv(n, 256 / NL)), dim3(256), 0, st, static_cast<const T*>(in->x),
+                       static_cast<const T*>(in->delta), in->A, static_cast<const T*>(in->B), static_cast<const T*>(in->C), in->D,
+                       static_cast<const T*>(in->z), in->delta_bias, state, state_out, y, n, s->D, s->G, s->N, s->delta_softplus);
+    RST_LAUNCH_CHECK();
+    return RST_OK;
+}
+
+}  // namespace rst
+
+using namespace rst;
+
+#define SCAN_WAVES(CALL, T) (W == 1 ? CALL(T, 1) : W == 2 ? CALL(T, 2) : W == 4 ? CALL(T, 4) : CALL(T, 8))
+#define SCAN_TYPES(CALL) (s->dtype == RST_DTYPE_F32 ? SCAN_WAVES(CALL, float) : SCAN_WAVES(CALL, bf16_t))
+
+extern "C" {
+
+size_t rst_scan_workspace_bytes(const rst_scan_desc* s) {
+    if (scan_check("scan_workspace_bytes", s) != RST_OK) return 0;
+    Scan a{};
+    scan_shape(&a, s);
+    return scan_carve(&a, nullptr, false);
+}
+size_t rst_scan_saved_bytes(const rst_scan_desc* s) {
+    if (scan_check("scan_saved_bytes", s) != RST_OK) return 0;
+    Scan a{};
+    scan_shape(&a, s);
+    return (size_t)a.B * a.tiles * 4 * scan_waves(a.N) * a.D * sizeof(float);
+}
+size_t rst_scan_bwd_workspace_bytes(const rst_scan_desc* s) {
+    if (scan_check("scan_bwd_workspace_bytes", s) != RST_OK) return 0;
+    Scan a{};
+    scan_shape(&a, s);
+    return scan_carve(&a, nullptr, true);
+}
+
+int rst_scan_fwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float* state_in, void* y, float* state_out, float* saved,
+                 void* workspace, size_t workspace_bytes, void* stream) {
+    RST_TRY(scan_check("scan_fwd", s));
+    RST_REQUIRE(in && in->x && in->delta && in->A && in->B && in->C && y, "scan_fwd: null operand");
+    Scan a{};
+    scan_shape(&a, s);
+    const size_t need = scan_carve(&a, nullptr, false);
+    if (workspace == nullptr || workspace_bytes < need)
+        return fail(RST_ERR_WORKSPACE, "scan_fwd: workspace too small (%zu < %zu)", workspace_bytes, need);
+    RST_REQUIRE(aligned16(workspace), "scan_fwd: workspace not aligned to 16 bytes");
+    scan_carve(&a, static_cast<char*>(workspace), false);
+    a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
+    a.h0 = state_in; a.y = y; a.last = state_out; a.ckpt = saved;
+    const int W = scan_waves(a.N);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define FWD(T, W_) scan_fwd_t<T, W_>(a, st)
+    return SCAN_TYPES(FWD);
+#undef FWD
+}
+
+int rst_scan_bwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float* saved, const void* dy, const float* dstate_out,
+                 const rst_scan_grads* out, float* dstate_in, void* workspace, size_t workspace_bytes, void* stream) {
+    RST_TRY(scan_check("scan_bwd", s));
+    RST_REQUIRE(in && in->x && in->delta && in->A && in->B && in->C && saved && dy, "scan_bwd: null operand");
+    RST_REQUIRE(out && out->x && out->delta && out->A && out->B && out->C && (!in->z || out->z), "scan_bwd: null gradient");
+    Scan a{};
+    scan_shape(&a, s);
+    const size_t need = scan_carve(&a, nullptr, true);
+    if (workspace == nullptr || workspace_bytes < need)
+        return fail(RST_ERR_WORKSPACE, "scan_bwd: workspace too small (%zu < %zu)", workspace_bytes, need);
+    RST_REQUIRE(aligned16(workspace), "scan_bwd: workspace not aligned to 16 bytes");
+    scan_carve(&a, static_cast<char*>(workspace), true);
+    a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
+    a.ckpt = const_cast<float*>(saved); a.dy = dy; a.dlast = dstate_out;
+    a.dx = out->x; a.ddelta = out->delta; a.dB = out->B; a.dC = out->C; a.dz = out->z; a.dh0 = dstate_in;
+    const int W = scan_waves(a.N);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define BWD(T, W_) scan_bwd_t<T, W_>(a, out->A, out->D, out->delta_bias, st)
+    return SCAN_TYPES(BWD);
+#undef BWD
+}
+
+int rst_scan_update(const rst_scan_desc* s, const rst_scan_inputs* in, const float* state_in, float* state_out, void* y, void* stream) {
+    RST_TRY(scan_check("scan_update", s));
+    RST_REQUIRE(s->L == 1, "scan_update: one token, not %lld", (long long)s->L);
+    RST_REQUIRE(in && in->x && in->delta && in->A && in->B && in->C && y && state_in && state_out, "scan_update: null operand");
+    const int W = scan_waves(s->N);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define UPD(T, NL) scan_update_t<T, NL>(s, in, state_in, state_out, static_cast<T*>(y), st)
+    return SCAN_TYPES(UPD);
+#undef UPD
+}
+
+}  // extern "C"

@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .. import ops
+from .. import ops, sequence
 
 
 def _flat(conv: nn.Conv2d):
@@ -44,7 +44,8 @@ def to_4d(x, h, w):
 class _ChannelNormBase(nn.Module):
     """Holds ``weight`` (and ``bias``) of shape (C,).  ``forward`` follows the
     reference bodies, which take the (b, hw, c) view (model/Restromer.py:40-42,
-    58-61); LayerNorm below calls the NCHW kernel directly instead."""
+    58-61); LayerNorm below calls the NCHW kernel directly instead.  bf16 tokens
+    go to the row kernel (sequence.layernorm), which has that type."""
     with_bias = False
 
     def __init__(self, normalized_shape):
@@ -60,6 +61,8 @@ class _ChannelNormBase(nn.Module):
         self.normalized_shape = normalized_shape
 
     def forward(self, x):
+        if x.dtype == torch.bfloat16:
+            return sequence.layernorm(x, self.weight, self.bias if self.with_bias else None)
         # x: (b, hw, c)  ->  NCHW with W = 1, run the kernel, and back
         b, n, c = x.shape
         y = ops.layernorm(x.transpose(1, 2).reshape(b, c, n, 1), self.weight, self.bias if self.with_bias else None)
