@@ -38,7 +38,7 @@ struct Scan {
     float* ckpt;                        // [B][tiles][4 W][D]: the state at every tile's start, or null
     float* cst;                         // [B][chunks][4 W][D]: what a chunk adds to the state behind (backward: before) it
     float* cdt;                         // [B][chunks][D]: sum of dt
-    float* bcpart;                      // [channel blocks of a group][B][G][tiles * 16][W][8]: shares of dB and dC
+    float* bcpart;                      // [channel blocks of a group][B][G][tiles * 2][W][64]: shares of dB and dC (tokens_fold)
     float* dApart;                      // [B][chunks][4 W][D]
     float* dDpart;                      // [B][chunks][2][D]: dD, dbias
     int B, D, G, N, Dg, cb;             // cb: channel blocks of a group
@@ -72,37 +72,38 @@ struct ScanPlace {
     }
 };
 
-// four tokens of one channel
+// four tokens of one channel; `full`: the tile ends within the row (the same for the whole block, so no branch)
 template <typename T> struct Quad {
     Raw<T, 4> r;
-    __device__ __forceinline__ void load(const T* row, int64_t t, int64_t L, bool ok) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(r.w) / 4); ++i) r.w[i] = 0;
-        if (!ok) return;
-        if (t + 4 <= L) { r.load(row + t); return; }
+    __device__ __forceinline__ void load(const void* tensor, int64_t row, int64_t t, int64_t L, bool full) {
+        const T* p = static_cast<const T*>(tensor) + row;
+        if (full) { r.load(p + t); return; }
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = t + i < L ? Store<T>::get(row[t + i]) : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = t + i < L ? Store<T>::get(p[t + i]) : 0.f;
         r.pack(v);
     }
-    static __device__ __forceinline__ void put(T* row, int64_t t, int64_t L, bool ok, const float (&v)[4]) {
+    static __device__ __forceinline__ void put(void* tensor, int64_t row, int64_t t, int64_t L, bool full, bool ok, const float (&v)[4]) {
         if (!ok) return;
-        if (t + 4 <= L) {
+        T* p = static_cast<T*>(tensor) + row;
+        if (full) {
             Raw<T, 4> o;
             o.pack(v);
-            o.store(row + t);
+            o.store(p + t);
             return;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (t + i < L) row[t + i] = Store<T>::put(v[i]);
+            if (t + i < L) p[t + i] = Store<T>::put(v[i]);
     }
 };
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 // a block of W waves has 64 channels x 4 quads of a tile to load: items per thread
 template <int W> struct ScanItems { static constexpr int N = W >= 4 ? 1 : 4 / W; };
 
-// the channel, quad and address of one of a thread's items
+// the channel, quad and address of one of a thread's items; a thread without one reads channel 0 and writes nothing
 template <int W> struct ScanItem {
     int r, q, d; bool ok; int64_t row;
     __device__ __forceinline__ ScanItem() {}
@@ -114,7 +115,7 @@ template <int W> struct ScanItem {
         ok = i < 256 && p.cb * SC + r < a.Dg;
         row = ((int64_t)p.b * a.D + (ok ? d : 0)) * a.L;
     }
-    static __device__ __forceinline__ bool has(int k) { return threadIdx.x + k * 64 * W < 256; }
+    static __device__ __forceinline__ bool has(int k) { return W <= 4 || threadIdx.x < 256; }
 };
 
 __device__ __forceinline__ float step_size(const Scan& a, float raw) { return a.softplus ? softplus(raw) : raw; }
@@ -148,8 +149,25 @@ __device__ __forceinline__ void load_rates(const Scan& a, int d, bool ok, int wa
     for (int s = 0; s < 4; ++s) A[s] = ok && wave * 4 + s < a.N ? a.A[(int64_t)d * a.N + wave * 4 + s] : 0.f;
 }
 
+// dt of four tokens: zero where there is no channel or token, so that nothing there moves a state
+template <typename T>
+__device__ __forceinline__ void step_sizes(const Scan& a, const Quad<T>& q, float bias, int64_t t, bool full, bool ok, float (&raw)[4],
+                                           float (&dt)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        raw[i] = q.r.get(i) + bias;
+        const float v = step_size(a, raw[i]);
+        dt[i] = ok && (full || t + i < a.L) ? v : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ float gate_of(const Quad<T>& z, int i) {
+    const float v = z.r.get(i);
+    return v * sigmoid(v);
+}
+
 // ---- what a chunk adds to the state behind it (REV: to the state's gradient before it), and the sum of its dt -------
-template <typename T, int W, bool REV>
+template <typename T, int W, bool Z, bool REV>
 __global__ void __launch_bounds__(64 * W)
 scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     constexpr int NI = ScanItems<W>::N;
@@ -162,49 +180,59 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) A[s] *= LOG2E;
     const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
-    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave) * 8;
+    const f32x8* bc = reinterpret_cast<const f32x8*>(bc0) + (int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave;
     ScanItem<W> it[NI];
     float bias[NI];
+    Quad<T> qd[NI], qx[NI], qz[NI];
+    auto fetch = [&](int tile) {
+        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
+            qd[k].load(a.delta, it[k].row, t, a.L, full);
+            qx[k].load(REV ? a.dy : a.x, it[k].row, t, a.L, full);
+            if constexpr (REV && Z) qz[k].load(a.z, it[k].row, t, a.L, full);
+        }
+    };
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
         it[k].set(a, p, k);
         bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
     }
+    fetch(REV ? t1 - 1 : t0);
     for (int n = 0; n < t1 - t0; ++n) {
         const int tile = REV ? t1 - 1 - n : t0 + n;
+        const bool full = (int64_t)(tile + 1) * ST <= a.L;
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
-            Quad<T> qd, qx, qz;
-            qd.load(static_cast<const T*>(a.delta) + it[k].row, t, a.L, it[k].ok);
-            qx.load(static_cast<const T*>(REV ? a.dy : a.x) + it[k].row, t, a.L, it[k].ok);
-            if (REV && a.z) qz.load(static_cast<const T*>(a.z) + it[k].row, t, a.L, it[k].ok);
+            float raw[4], dt[4];
+            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw, dt);
             if (ScanItem<W>::has(k)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float dt = it[k].ok && t + i < a.L ? step_size(a, qd.r.get(i) + bias[k]) : 0.f;
-                    float u;
-                    if (REV) {
-                        u = qx.r.get(i);
-                        if (a.z) { const float z = qz.r.get(i); u *= z * sigmoid(z); }
-                    } else u = dt * qx.r.get(i);
-                    dts[it[k].q * 4 + i][it[k].r] = dt;
+                    float u = qx[k].r.get(i);
+                    if constexpr (REV) {
+                        if constexpr (Z) u *= gate_of(qz[k], i);
+                        u = it[k].ok ? u : 0.f;
+                    } else u *= dt[i];
+                    dts[it[k].q * 4 + i][it[k].r] = dt[i];
                     us[it[k].q * 4 + i][it[k].r] = u;
                 }
             }
         }
+        if (n + 1 < t1 - t0) fetch(REV ? tile - 1 : tile + 1);
         __syncthreads();
-        const float* bt = bc + (int64_t)tile * ST * W * 8;
-#pragma unroll 4
+        const f32x8* bt = bc + (int64_t)tile * ST * W;
+#pragma unroll 8
         for (int i = 0; i < ST; ++i) {
             const int tt = REV ? ST - 1 - i : i;
-            const float* v = bt + tt * W * 8;
+            const f32x8 v = bt[tt * W];
             const float dt = dts[tt][p.lane], u = us[tt][p.lane];
             sum += dt;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const float decay = __builtin_amdgcn_exp2f(dt * A[s]);
-                if (REV) h[s] = decay * fmaf(u, v[4 + s], h[s]);
+                if constexpr (REV) h[s] = decay * fmaf(u, v[4 + s], h[s]);
                 else h[s] = fmaf(decay, h[s], u * v[s]);
             }
         }
@@ -219,7 +247,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
-template <typename T, int W>
+template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W)
 scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
     constexpr int NI = ScanItems<W>::N;
@@ -227,6 +255,27 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
     const ScanPlace p(a, a.nchunk, 0);
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
     const bool ok = p.cb * SC + p.lane < a.Dg;
+    const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
+    ScanItem<W> it[NI];
+    float bias[NI], skip[NI];
+    Quad<T> qd[NI], qx[NI], qz[NI];
+    auto fetch = [&](int tile) {
+        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
+            qd[k].load(a.delta, it[k].row, t, a.L, full);
+            qx[k].load(a.x, it[k].row, t, a.L, full);
+            if constexpr (Z) qz[k].load(a.z, it[k].row, t, a.L, full);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+        it[k].set(a, p, k);
+        bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
+        skip[k] = a.Dskip && it[k].ok ? a.Dskip[it[k].d] : 0.f;
+    }
+    fetch(t0);
     float A[4], h[4];
     load_rates(a, d, ok, p.wave, A);
 #pragma unroll
@@ -234,53 +283,44 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
         A[s] *= LOG2E;
         h[s] = a.h0 && ok && p.wave * 4 + s < a.N ? a.h0[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
     }
+    const int dr = ok ? d : 0;
+#pragma unroll 4
     for (int c = 0; c < p.chunk; ++c) {
         const int64_t ci = (int64_t)p.b * a.nchunk + c;
-        const float sum = ok ? a.cdt[ci * a.D + d] : 0.f;
+        const float sum = a.cdt[ci * a.D + dr];
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-            h[s] = fmaf(__builtin_amdgcn_exp2f(sum * A[s]), h[s], ok ? a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + d] : 0.f);
+            h[s] = fmaf(__builtin_amdgcn_exp2f(sum * A[s]), h[s], a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + dr]);
     }
-    const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
-    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave) * 8;
-    ScanItem<W> it[NI];
-    float bias[NI], skip[NI];
-#pragma unroll
-    for (int k = 0; k < NI; ++k) {
-        it[k].set(a, p, k);
-        bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
-        skip[k] = a.Dskip && it[k].ok ? a.Dskip[it[k].d] : 0.f;
-    }
+    const f32x8* bc = reinterpret_cast<const f32x8*>(bc0) + (int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave;
     for (int tile = t0; tile < t1; ++tile) {
-        float x[NI][4];
-        Quad<T> qz[NI];
+        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        float x[NI][4], gate[NI][4];
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
-            Quad<T> qd, qx;
-            qd.load(static_cast<const T*>(a.delta) + it[k].row, t, a.L, it[k].ok);
-            qx.load(static_cast<const T*>(a.x) + it[k].row, t, a.L, it[k].ok);
-            if (a.z) qz[k].load(static_cast<const T*>(a.z) + it[k].row, t, a.L, it[k].ok);
+            float raw[4], dt[4];
+            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw, dt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float dt = it[k].ok && t + i < a.L ? step_size(a, qd.r.get(i) + bias[k]) : 0.f;
-                x[k][i] = qx.r.get(i);
+                x[k][i] = qx[k].r.get(i);
+                if constexpr (Z) gate[k][i] = gate_of(qz[k], i);
                 if (ScanItem<W>::has(k)) {
-                    dts[it[k].q * 4 + i][it[k].r] = dt;
-                    us[it[k].q * 4 + i][it[k].r] = dt * x[k][i];
+                    dts[it[k].q * 4 + i][it[k].r] = dt[i];
+                    us[it[k].q * 4 + i][it[k].r] = dt[i] * x[k][i];
                 }
             }
         }
+        if (tile + 1 < t1) fetch(tile + 1);
         __syncthreads();
         if (a.ckpt && ok) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + d] = h[s];
         }
-        const float* bt = bc + (int64_t)tile * ST * W * 8;
-#pragma unroll 4
+        const f32x8* bt = bc + (int64_t)tile * ST * W;
+#pragma unroll 8
         for (int i = 0; i < ST; ++i) {
-            const float* v = bt + i * W * 8;
+            const f32x8 v = bt[i * W];
             const float dt = dts[i][p.lane], u = us[i][p.lane];
             float y = 0.f;
 #pragma unroll
@@ -297,13 +337,12 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float s = skip[k] * x[k][i];
+                y[i] = skip[k] * x[k][i];
 #pragma unroll
-                for (int w = 0; w < W; ++w) s += part[w][it[k].q * 4 + i][it[k].r];
-                if (a.z) { const float z = qz[k].r.get(i); s *= z * sigmoid(z); }
-                y[i] = s;
+                for (int w = 0; w < W; ++w) y[i] += part[w][it[k].q * 4 + i][it[k].r];
+                if constexpr (Z) y[i] *= gate[k][i];
             }
-            Quad<T>::put(static_cast<T*>(a.y) + it[k].row, (int64_t)tile * ST + it[k].q * 4, a.L, it[k].ok, y);
+            Quad<T>::put(a.y, it[k].row, (int64_t)tile * ST + it[k].q * 4, a.L, full, it[k].ok, y);
         }
     }
     if (a.last && ok && t1 == a.tiles) {
@@ -314,37 +353,55 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-template <typename T, int W>
-__global__ void __launch_bounds__(64 * W)
-scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
+// Sums over the 64 lanes, many values at a time: where a butterfly would add a value to itself in both halves, two
+// values swap halves first, so that every step halves the number of values (8 values of 8 tokens: 141 instructions
+// instead of 384 for 64 butterflies).
+__device__ __forceinline__ float halves32(float a, float b) {              // lanes 0-31: a's sum, 32-63: b's
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float halves16(float a, float b) {              // even rows of 16 lanes: a's, odd rows: b's
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// lanes with `hi` unset: a's sum with the lane that CTRL names, with it set: b's
+template <int CTRL> __device__ __forceinline__ float halves_dpp(float a, float b, bool hi) {
+    return (hi ? b : a) + dpp<CTRL>(hi ? a : b);
+}
+constexpr int DPP_ROR8 = 0x128, DPP_HALF_MIRROR = 0x141, DPP_XOR2 = 0x4E, DPP_XOR1 = 0xB1;
+// the shares of dB (v[0..3]) and dC (v[4..7]) of one token: lane l holds value 4 (l >> 5) + 2 (l >> 4 & 1) + (l >> 3 & 1),
+// still to be added over its group of eight lanes
+__device__ __forceinline__ float lanes_fold(const float (&v)[8], int lane) {
+    float h[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) h[s] = halves32(v[s], v[4 + s]);
+    return halves_dpp<DPP_ROR8>(halves16(h[0], h[2]), halves16(h[1], h[3]), lane & 8);
+}
+// those of eight tokens: lane l holds the finished value of token l & 7
+__device__ __forceinline__ float tokens_fold(const float (&w)[8], int lane) {
+    float q[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = halves_dpp<DPP_HALF_MIRROR>(w[k], w[k + 4], lane & 4);
+    return halves_dpp<DPP_XOR1>(halves_dpp<DPP_XOR2>(q[0], q[2], lane & 2), halves_dpp<DPP_XOR2>(q[1], q[3], lane & 2), lane & 1);
+}
+
+// WHOLE: the block has 64 channels.  Where it has fewer, the shares of the lanes without one are taken out: they are
+// zero only as long as B and C are finite.
+template <typename T, int W, bool Z, bool WHOLE>
+__device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __restrict__ bc0, const ScanPlace& p, float* smem) {
     constexpr int NI = ScanItems<W>::N;
-    extern __shared__ __attribute__((aligned(16))) float smem[];
     float (*dts)[SROW] = reinterpret_cast<float (*)[SROW]>(smem);
     float (*us)[SROW] = dts + ST;
     float (*es)[SROW] = us + ST;
     float (*part0)[ST][SROW] = reinterpret_cast<float (*)[ST][SROW]>(es + ST);          // [W]: shares of s, then of sum g B
     float (*part1)[ST][SROW] = part0 + W;                                               // [W]: shares of sum A a g h
-    const ScanPlace p(a, a.nchunk, 0);
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
-    const bool ok = p.cb * SC + p.lane < a.Dg;
-    float A[4], A2[4], g[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
-    load_rates(a, d, ok, p.wave, A);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        A2[s] = A[s] * LOG2E;
-        g[s] = a.dlast && ok && p.wave * 4 + s < a.N ? a.dlast[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
-    }
-    for (int c = a.nchunk - 1; c > p.chunk; --c) {
-        const int64_t ci = (int64_t)p.b * a.nchunk + c;
-        const float sum = ok ? a.cdt[ci * a.D + d] : 0.f;
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            g[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), g[s], ok ? a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + d] : 0.f);
-    }
+    const bool ok = WHOLE || p.cb * SC + p.lane < a.Dg;
+    const int dr = ok ? d : 0;
     const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
-    const int64_t bg = (int64_t)p.b * a.G + p.g;
-    const float* bc = bc0 + (bg * a.tiles * ST * W + p.wave) * 8;
-    float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * ST * W + p.wave) * 8;
     ScanItem<W> it[NI];
     float bias[NI], skip[NI], dD[NI], db[NI];
 #pragma unroll
@@ -355,24 +412,55 @@ scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
         dD[k] = 0.f;
         db[k] = 0.f;
     }
-    for (int tile = t1 - 1; tile >= t0; --tile) {
-        float x[NI][4], dt[NI][4], e[NI][4], raw[NI][4];
-        Quad<T> qz[NI], qy[NI];
+    Quad<T> qd[NI], qx[NI], qy[NI], qz[NI];
+    float hn[4];
+    auto fetch = [&](int tile) {
+        const bool full = (int64_t)(tile + 1) * ST <= a.L;
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             const int64_t t = (int64_t)tile * ST + it[k].q * 4;
-            Quad<T> qd, qx;
-            qd.load(static_cast<const T*>(a.delta) + it[k].row, t, a.L, it[k].ok);
-            qx.load(static_cast<const T*>(a.x) + it[k].row, t, a.L, it[k].ok);
-            qy[k].load(static_cast<const T*>(a.dy) + it[k].row, t, a.L, it[k].ok);
-            if (a.z) qz[k].load(static_cast<const T*>(a.z) + it[k].row, t, a.L, it[k].ok);
+            qd[k].load(a.delta, it[k].row, t, a.L, full);
+            qx[k].load(a.x, it[k].row, t, a.L, full);
+            qy[k].load(a.dy, it[k].row, t, a.L, full);
+            if constexpr (Z) qz[k].load(a.z, it[k].row, t, a.L, full);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) hn[s] = a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + dr];
+    };
+    fetch(t1 - 1);
+    float A[4], A2[4], g[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
+    load_rates(a, d, ok, p.wave, A);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        A2[s] = A[s] * LOG2E;
+        g[s] = a.dlast && ok && p.wave * 4 + s < a.N ? a.dlast[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
+    }
+#pragma unroll 4
+    for (int c = a.nchunk - 1; c > p.chunk; --c) {
+        const int64_t ci = (int64_t)p.b * a.nchunk + c;
+        const float sum = a.cdt[ci * a.D + dr];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            g[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), g[s], a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + dr]);
+    }
+    const int64_t bg = (int64_t)p.b * a.G + p.g;
+    const f32x8* bc = reinterpret_cast<const f32x8*>(bc0) + bg * a.tiles * ST * W + p.wave;
+    float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * 2 * W + p.wave) * 64 + p.lane;
+    for (int tile = t1 - 1; tile >= t0; --tile) {
+        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        float x[NI][4], dt[NI][4], e[NI][4], raw[NI][4], slope[NI][4];          // slope: dy silu'(z)
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw[k], dt[k]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                raw[k][i] = qd.r.get(i) + bias[k];
-                dt[k][i] = it[k].ok && t + i < a.L ? step_size(a, raw[k][i]) : 0.f;
-                x[k][i] = qx.r.get(i);
-                e[k][i] = qy[k].r.get(i);
-                if (a.z) { const float z = qz[k].r.get(i); e[k][i] *= z * sigmoid(z); }
+                x[k][i] = qx[k].r.get(i);
+                e[k][i] = it[k].ok ? qy[k].r.get(i) : 0.f;
+                if constexpr (Z) {
+                    const float z = qz[k].r.get(i), q = sigmoid(z);
+                    slope[k][i] = e[k][i] * (q * fmaf(z, 1.0f - q, 1.0f));
+                    e[k][i] *= z * q;
+                }
                 if (ScanItem<W>::has(k)) {
                     dts[it[k].q * 4 + i][it[k].r] = dt[k][i];
                     us[it[k].q * 4 + i][it[k].r] = dt[k][i] * x[k][i];
@@ -382,43 +470,44 @@ scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
         }
         float hs[ST + 1][4], as[ST][4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-            hs[0][s] = ok ? a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + d] : 0.f;
+        for (int s = 0; s < 4; ++s) hs[0][s] = ok ? hn[s] : 0.f;
+        if (tile > t0) fetch(tile - 1);
         __syncthreads();
-        const float* bt = bc + (int64_t)tile * ST * W * 8;
+        const f32x8* bt = bc + (int64_t)tile * ST * W;
 #pragma unroll
         for (int i = 0; i < ST; ++i) {
-            const float* v = bt + i * W * 8;
+            const f32x8 v = bt[i * W];
             const float dti = dts[i][p.lane], u = us[i][p.lane];
             float y = 0.f;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 as[i][s] = __builtin_amdgcn_exp2f(dti * A2[s]);
                 hs[i + 1][s] = fmaf(as[i][s], hs[i][s], u * v[s]);
-                if (a.z) y = fmaf(v[4 + s], hs[i + 1][s], y);
+                if constexpr (Z) y = fmaf(v[4 + s], hs[i + 1][s], y);
             }
-            if (a.z) part0[p.wave][i][p.lane] = y;
+            if constexpr (Z) part0[p.wave][i][p.lane] = y;
         }
-        float dz[NI][4];
-        if (a.z) {
+        if constexpr (Z) {
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < NI; ++k)
+            for (int k = 0; k < NI; ++k) {
+                if (!ScanItem<W>::has(k)) continue;
+                float dz[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (!ScanItem<W>::has(k)) continue;
-                    float s = skip[k] * x[k][i];
+                    float y = skip[k] * x[k][i];
 #pragma unroll
-                    for (int w = 0; w < W; ++w) s += part0[w][it[k].q * 4 + i][it[k].r];
-                    const float z = qz[k].r.get(i), q = sigmoid(z);
-                    dz[k][i] = qy[k].r.get(i) * s * (q * fmaf(z, 1.0f - q, 1.0f));
+                    for (int w = 0; w < W; ++w) y += part0[w][it[k].q * 4 + i][it[k].r];
+                    dz[i] = slope[k][i] * y;
                 }
+                Quad<T>::put(a.dz, it[k].row, (int64_t)tile * ST + it[k].q * 4, a.L, full, it[k].ok, dz);
+            }
             __syncthreads();
         }
-        float tA[4] = {0.f, 0.f, 0.f, 0.f};
+        float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
 #pragma unroll
         for (int i = ST - 1; i >= 0; --i) {
-            const float* v = bt + i * W * 8;
+            const f32x8 v = bt[i * W];
             const float dti = dts[i][p.lane], u = us[i][p.lane], ei = es[i][p.lane];
             float gB = 0.f, gA = 0.f, pr[8];
 #pragma unroll
@@ -434,11 +523,12 @@ scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
             }
             part0[p.wave][i][p.lane] = gB;
             part1[p.wave][i][p.lane] = gA;
+            if constexpr (!WHOLE) {
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const float v8 = wave_sum(ok ? pr[s] : 0.f);       // (no channel there: 0 times an infinite C is no zero)
-                if (p.lane == s) bco[((int64_t)tile * ST + i) * W * 8 + s] = v8;
+                for (int s = 0; s < 8; ++s) pr[s] = ok ? pr[s] : 0.f;
             }
+            fold[i & 7] = lanes_fold(pr, p.lane);
+            if ((i & 7) == 0) bco[((int64_t)tile * 2 + (i >> 3)) * W * 64] = tokens_fold(fold, p.lane);
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) dA[s] += tA[s];
@@ -459,14 +549,13 @@ scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
                 ox[i] = fmaf(gB, dt[k][i], skip[k] * e[k][i]);
                 od[i] = fmaf(gB, x[k][i], gA);
                 if (a.softplus) od[i] *= sigmoid(raw[k][i]);
-                if (it[k].ok && t + i < a.L) {
+                if (full || t + i < a.L) {
                     dD[k] = fmaf(e[k][i], x[k][i], dD[k]);
                     db[k] += od[i];
                 }
             }
-            Quad<T>::put(static_cast<T*>(a.dx) + it[k].row, t, a.L, it[k].ok, ox);
-            Quad<T>::put(static_cast<T*>(a.ddelta) + it[k].row, t, a.L, it[k].ok, od);
-            if (a.z) Quad<T>::put(static_cast<T*>(a.dz) + it[k].row, t, a.L, it[k].ok, dz[k]);
+            Quad<T>::put(a.dx, it[k].row, t, a.L, full, it[k].ok, ox);
+            Quad<T>::put(a.ddelta, it[k].row, t, a.L, full, it[k].ok, od);
         }
         __syncthreads();
     }
@@ -492,30 +581,33 @@ scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
     }
 }
 
-// dB, dC [B][G][N][L]: the channel blocks' shares in a fixed order, turned back to token-contiguous
+template <typename T, int W, bool Z>
+__global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)
+scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
+    extern __shared__ __attribute__((aligned(16))) float smem[];
+    const ScanPlace p(a, a.nchunk, 0);
+    if (p.cb * SC + SC <= a.Dg) scan_bwd_body<T, W, Z, true>(a, bc0, p, smem);
+    else scan_bwd_body<T, W, Z, false>(a, bc0, p, smem);
+}
+
+// dB, dC [B][G][N][L]: the channel blocks' shares in a fixed order, turned back to token-contiguous.  A thread has one
+// token and one state.
 template <typename T>
 __global__ void __launch_bounds__(256)
 scan_reduce_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC, int cb, int64_t stride, int N, int W,
-                      int64_t L, int64_t Lp) {
+                      int64_t L, int64_t groups) {
     const int64_t t = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     const int64_t bg = blockIdx.y;
     if (t >= L) return;
-    for (int w = threadIdx.x >> 6; w < W; w += 4) {
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int c = 0; c < cb; ++c) {
-            Raw<float, 8> v;
-            v.load(part + c * stride + ((bg * Lp + t) * W + w) * 8);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += v.get(i);
+    for (int n = threadIdx.x >> 6; n < N; n += 4) {
+        const float* p = part + ((bg * groups + (t >> 3)) * W + (n >> 2)) * 64 + ((n >> 1) & 1) * 16 + (n & 1) * 8 + (t & 7);
+        float b = 0.f, c = 0.f;
+        for (int k = 0; k < cb; ++k) {
+            b += p[k * stride];
+            c += p[k * stride + 32];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = w * 4 + i;
-            if (n < N) {
-                dB[(bg * N + n) * L + t] = Store<T>::put(s[i]);
-                dC[(bg * N + n) * L + t] = Store<T>::put(s[4 + i]);
-            }
-        }
+        dB[(bg * N + n) * L + t] = Store<T>::put(b);
+        dC[(bg * N + n) * L + t] = Store<T>::put(c);
     }
 }
 
@@ -603,6 +695,7 @@ scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const f
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
+static bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
 static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 
 // Chunks: enough blocks for two of them on each of the 256 compute units, chunks of at least four tiles.
@@ -666,7 +759,7 @@ static int scan_prep(const Scan& a, int W, hipStream_t st) {
     return RST_OK;
 }
 
-template <typename T, int W>
+template <typename T, int W, bool Z>
 static int scan_fwd_t(const Scan& a, hipStream_t st) {
     const double n = (double)a.B * a.D * a.L;
     ProfScope prof(st, "scan_fwd", n * (7.0 * a.N + 12), sizeof(T) * n * (a.z ? 4 : 3));
@@ -674,15 +767,15 @@ static int scan_fwd_t(const Scan& a, hipStream_t st) {
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
         RST_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, W>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a, a.bc);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a, a.bc);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
 
-template <typename T, int W>
+template <typename T, int W, bool Z>
 static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStream_t st) {
     const double n = (double)a.B * a.D * a.L;
     ProfScope prof(st, "scan_bwd", n * (16.0 * a.N + 28), sizeof(T) * n * (a.z ? 7 : 5));
@@ -690,17 +783,16 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, W, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
         RST_LAUNCH_CHECK();
     }
     const size_t lds = (size_t)(3 + 2 * W) * ST * SROW * sizeof(float);
     KernelSetup ks;
-    RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W>), 64 * W, lds, &ks));
-    hipLaunchKernelGGL((scan_bwd_kernel<T, W>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a, a.bc);
+    RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W, Z>), 64 * W, lds, &ks));
+    hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a, a.bc);
     RST_LAUNCH_CHECK();
-    const int64_t Lp = (int64_t)a.tiles * ST;
     hipLaunchKernelGGL((scan_reduce_bc_kernel<T>), dim3((unsigned)cdiv(a.L, 64), a.B * a.G), dim3(256), 0, st, a.bcpart,
-                       static_cast<T*>(a.dB), static_cast<T*>(a.dC), a.cb, (int64_t)a.B * a.G * Lp * W * 8, a.N, W, a.L, Lp);
+                       static_cast<T*>(a.dB), static_cast<T*>(a.dC), a.cb, (int64_t)a.B * a.G * a.tiles * 2 * W * 64, a.N, W, a.L, (int64_t)a.tiles * 2);
     RST_LAUNCH_CHECK();
     hipLaunchKernelGGL(scan_reduce_params_kernel, dim3((unsigned)cdiv(a.D, 16), a.N + 2), dim3(256), 0, st, a.dApart, a.dDpart, dA, dD,
                        dbias, a.B * a.nchunk, a.D, a.N, W);
@@ -756,13 +848,13 @@ int rst_scan_fwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     const size_t need = scan_carve(&a, nullptr, false);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_fwd: workspace too small (%zu < %zu)", workspace_bytes, need);
-    RST_REQUIRE(aligned16(workspace), "scan_fwd: workspace not aligned to 16 bytes");
+    RST_REQUIRE(aligned256(workspace), "scan_fwd: workspace not aligned to 256 bytes");
     scan_carve(&a, static_cast<char*>(workspace), false);
     a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
     a.h0 = state_in; a.y = y; a.last = state_out; a.ckpt = saved;
     const int W = scan_waves(a.N);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define FWD(T, W_) scan_fwd_t<T, W_>(a, st)
+#define FWD(T, W_) (a.z ? scan_fwd_t<T, W_, true>(a, st) : scan_fwd_t<T, W_, false>(a, st))
     return SCAN_TYPES(FWD);
 #undef FWD
 }
@@ -777,14 +869,15 @@ int rst_scan_bwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     const size_t need = scan_carve(&a, nullptr, true);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_bwd: workspace too small (%zu < %zu)", workspace_bytes, need);
-    RST_REQUIRE(aligned16(workspace), "scan_bwd: workspace not aligned to 16 bytes");
+    RST_REQUIRE(aligned256(workspace), "scan_bwd: workspace not aligned to 256 bytes");
     scan_carve(&a, static_cast<char*>(workspace), true);
     a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
     a.ckpt = const_cast<float*>(saved); a.dy = dy; a.dlast = dstate_out;
     a.dx = out->x; a.ddelta = out->delta; a.dB = out->B; a.dC = out->C; a.dz = out->z; a.dh0 = dstate_in;
     const int W = scan_waves(a.N);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define BWD(T, W_) scan_bwd_t<T, W_>(a, out->A, out->D, out->delta_bias, st)
+#define BWD(T, W_)                                                                                                      \
+    (a.z ? scan_bwd_t<T, W_, true>(a, out->A, out->D, out->delta_bias, st) : scan_bwd_t<T, W_, false>(a, out->A, out->D, out->delta_bias, st))
     return SCAN_TYPES(BWD);
 #undef BWD
 }
