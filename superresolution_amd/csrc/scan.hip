@@ -396,8 +396,9 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
     float (*dts)[SROW] = reinterpret_cast<float (*)[SROW]>(smem);
     float (*us)[SROW] = dts + ST;
     float (*es)[SROW] = us + ST;
-    float (*part0)[ST][SROW] = reinterpret_cast<float (*)[ST][SROW]>(es + ST);          // [W]: shares of s, then of sum g B
+    float (*part0)[ST][SROW] = reinterpret_cast<float (*)[ST][SROW]>(es + ST);          // [W]: shares of sum g B
     float (*part1)[ST][SROW] = part0 + W;                                               // [W]: shares of sum A a g h
+    float (*part2)[ST][SROW] = part1 + W;                                               // [W], with z: shares of s
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
     const bool ok = WHOLE || p.cb * SC + p.lane < a.Dg;
     const int dr = ok ? d : 0;
@@ -485,24 +486,7 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                 hs[i + 1][s] = fmaf(as[i][s], hs[i][s], u * v[s]);
                 if constexpr (Z) y = fmaf(v[4 + s], hs[i + 1][s], y);
             }
-            if constexpr (Z) part0[p.wave][i][p.lane] = y;
-        }
-        if constexpr (Z) {
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < NI; ++k) {
-                if (!ScanItem<W>::has(k)) continue;
-                float dz[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float y = skip[k] * x[k][i];
-#pragma unroll
-                    for (int w = 0; w < W; ++w) y += part0[w][it[k].q * 4 + i][it[k].r];
-                    dz[i] = slope[k][i] * y;
-                }
-                Quad<T>::put(a.dz, it[k].row, (int64_t)tile * ST + it[k].q * 4, a.L, full, it[k].ok, dz);
-            }
-            __syncthreads();
+            if constexpr (Z) part2[p.wave][i][p.lane] = y;
         }
         float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
 #pragma unroll
@@ -556,6 +540,17 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
             }
             Quad<T>::put(a.dx, it[k].row, t, a.L, full, it[k].ok, ox);
             Quad<T>::put(a.ddelta, it[k].row, t, a.L, full, it[k].ok, od);
+            if constexpr (Z) {
+                float oz[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float y = skip[k] * x[k][i];
+#pragma unroll
+                    for (int w = 0; w < W; ++w) y += part2[w][it[k].q * 4 + i][it[k].r];
+                    oz[i] = slope[k][i] * y;
+                }
+                Quad<T>::put(a.dz, it[k].row, t, a.L, full, it[k].ok, oz);
+            }
         }
         __syncthreads();
     }
@@ -698,16 +693,23 @@ scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const f
 static bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
 static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 
-// Chunks: enough blocks for two of them on each of the 256 compute units, chunks of at least four tiles.
-static void scan_plan(Scan* a) {
+// How many chunks a row is cut into.  The chip holds 1024 blocks of the forward kernel (four to a compute unit) or 512 of
+// the backward kernel (two); more run in rounds, so 528 blocks take as long as 1024.  Chunks cost the pass over the
+// chunks' own states, 0.6 of the forward kernel's time and 0.2 of the backward's, and a few steps of a chain per chunk before
+// a block.  The number with the least rounds x tiles is taken, chunks of at least four tiles.
+static void scan_plan(Scan* a, bool bwd) {
     a->Dg = a->D / a->G;
     a->cb = (int)cdiv(a->Dg, SC);
     a->tiles = (int)cdiv(a->L, ST);
-    const int64_t blocks = (int64_t)a->B * a->G * a->cb;
-    int64_t want = cdiv(512, blocks);
-    const int64_t most = a->tiles / 4 > 1 ? a->tiles / 4 : 1;
-    if (want > most) want = most;
-    a->per_chunk = (int)cdiv(a->tiles, want);
+    const int64_t blocks = (int64_t)a->B * a->G * a->cb, slots = bwd ? 512 : 1024;
+    const double again = bwd ? 1.2 : 1.6;
+    double best = (double)cdiv(blocks, slots) * a->tiles;
+    a->per_chunk = a->tiles;
+    for (int64_t n = 2; n <= a->tiles / 4 && n <= 256 && blocks * n <= 4 * slots; ++n) {
+        const int64_t per = cdiv(a->tiles, n), real = cdiv(a->tiles, per);
+        const double cost = (double)cdiv(blocks * real, slots) * per * again + 0.05 * real;
+        if (cost < best) { best = cost; a->per_chunk = (int)per; }
+    }
     a->nchunk = (int)cdiv(a->tiles, a->per_chunk);
 }
 
@@ -722,9 +724,9 @@ static int scan_check(const char* what, const rst_scan_desc* s) {
     return RST_OK;
 }
 
-static void scan_shape(Scan* a, const rst_scan_desc* s) {
+static void scan_shape(Scan* a, const rst_scan_desc* s, bool bwd) {
     a->B = s->B; a->D = s->D; a->G = s->G; a->N = s->N; a->L = s->L; a->softplus = s->delta_softplus;
-    scan_plan(a);
+    scan_plan(a, bwd);
 }
 
 // Scratch of a call, carved from the caller's workspace (base == null: only measured)
@@ -786,7 +788,7 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
         hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
         RST_LAUNCH_CHECK();
     }
-    const size_t lds = (size_t)(3 + 2 * W) * ST * SROW * sizeof(float);
+    const size_t lds = (size_t)(3 + (Z ? 3 : 2) * W) * ST * SROW * sizeof(float);
     KernelSetup ks;
     RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W, Z>), 64 * W, lds, &ks));
     hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a, a.bc);
@@ -823,19 +825,19 @@ extern "C" {
 size_t rst_scan_workspace_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_workspace_bytes", s) != RST_OK) return 0;
     Scan a{};
-    scan_shape(&a, s);
+    scan_shape(&a, s, false);
     return scan_carve(&a, nullptr, false);
 }
 size_t rst_scan_saved_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_saved_bytes", s) != RST_OK) return 0;
     Scan a{};
-    scan_shape(&a, s);
+    scan_shape(&a, s, true);
     return (size_t)a.B * a.tiles * 4 * scan_waves(a.N) * a.D * sizeof(float);
 }
 size_t rst_scan_bwd_workspace_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_bwd_workspace_bytes", s) != RST_OK) return 0;
     Scan a{};
-    scan_shape(&a, s);
+    scan_shape(&a, s, true);
     return scan_carve(&a, nullptr, true);
 }
 
@@ -844,7 +846,7 @@ int rst_scan_fwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     RST_TRY(scan_check("scan_fwd", s));
     RST_REQUIRE(in && in->x && in->delta && in->A && in->B && in->C && y, "scan_fwd: null operand");
     Scan a{};
-    scan_shape(&a, s);
+    scan_shape(&a, s, false);
     const size_t need = scan_carve(&a, nullptr, false);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_fwd: workspace too small (%zu < %zu)", workspace_bytes, need);
@@ -865,7 +867,7 @@ int rst_scan_bwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     RST_REQUIRE(in && in->x && in->delta && in->A && in->B && in->C && saved && dy, "scan_bwd: null operand");
     RST_REQUIRE(out && out->x && out->delta && out->A && out->B && out->C && (!in->z || out->z), "scan_bwd: null gradient");
     Scan a{};
-    scan_shape(&a, s);
+    scan_shape(&a, s, true);
     const size_t need = scan_carve(&a, nullptr, true);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_bwd: workspace too small (%zu < %zu)", workspace_bytes, need);
