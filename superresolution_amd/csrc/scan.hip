@@ -11,7 +11,7 @@
 // states: 96 operations for the 6 to 12 bytes of a bf16 or fp32 token), so the layout serves the instruction stream:
 //   - a lane is a channel and holds four of its states; the waves of a block hold the other states of the same 64
 //     channels.  B and C are then the same for a whole wave and come in as scalar operands (no vector register, no LDS).
-//     They are laid out for that once per call: [B][G][token][wave][B0..B3 C0..C3] in fp32 (bc_prep_kernel).
+//     They are laid out for that once per call: [B][G][wave][token][B0..B3 C0..C3] in fp32 (bc_prep_kernel).
 //   - tokens go in tiles of 16.  The tensors are token-contiguous, so a thread loads 4 tokens of one channel (a wave: 16
 //     channels x 16 tokens), takes softplus once, and hands dt and dt x over through LDS, turned to lane = channel; the
 //     waves' shares of s come back the same way.
@@ -34,7 +34,7 @@ struct Scan {
     const float *A, *Dskip, *dbias, *h0, *dlast;
     void *y, *dx, *ddelta, *dB, *dC, *dz;
     float *last, *dh0;
-    float* bc;                          // [B][G][tiles * 16][W][8]
+    float* bc;                          // [B][G][W][tiles * 16][8]
     float* ckpt;                        // [B][tiles][4 W][D]: the state at every tile's start, or null
     float* cst;                         // [B][chunks][4 W][D]: what a chunk adds to the state behind (backward: before) it
     float* cdt;                         // [B][chunks][D]: sum of dt
@@ -47,12 +47,16 @@ struct Scan {
     int softplus;
 };
 
-// log(1 + e^v): 1 + e^v loses the low bits of a small e^v, and log(w) e / (w - 1) gives them back
+// log(1 + e^v).  e^v: the rounding of v log2 e is given back (it is up to |v| 2^-24 of the result).  w = 1 + e^v loses the
+// low bits of a small e^v; below 1 they are worth c = e^v - (w - 1) itself (c / w up to one more rounding), above nothing.
 __device__ __forceinline__ float softplus(float v) {
-    if (v > 20.f) return v;
-    const float e = exp_near(v), w = 1.0f + e;
-    const float l = __builtin_amdgcn_logf(w) * 0.6931471805599453f;
-    return w == 1.0f ? e : l * e * rcp_fast(w - 1.0f);
+    const float t = v * LOG2E, low = fmaf(v, LOG2E, -t) * 0.6931471805599453f;
+    float e = __builtin_amdgcn_exp2f(t);
+    e = e > 0.f ? fmaf(e, low, e) : 0.f;                                   // (v = -inf: low is no number)
+    const float w = 1.0f + e;
+    const float c = e < 1.0f ? e - (w - 1.0f) : 0.f;
+    const float l = fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, c);
+    return v <= 20.f ? l : v;                                              // (and v itself where it is no number)
 }
 
 // which chunk, sample, group and channels a block has
@@ -98,7 +102,29 @@ template <typename T> struct Quad {
     }
 };
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+// B and C of four tokens and a wave's four states (scalar registers): token j's B is v[j / 2][8 (j % 2) + s], its C
+// v[j / 2][8 (j % 2) + 4 + s].
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+struct BC4 {
+    f32x16 v[2];
+    __device__ __forceinline__ void load(const float* __restrict__ bc, int64_t t) {
+        const f32x16* p = reinterpret_cast<const f32x16*>(bc + t * 8);
+        v[0] = p[0];
+        v[1] = p[1];
+    }
+    __device__ __forceinline__ float B(int j, int s) const { return v[j >> 1][(j & 1) * 8 + s]; }
+    __device__ __forceinline__ float C(int j, int s) const { return v[j >> 1][(j & 1) * 8 + 4 + s]; }
+};
+// Scalar loads come back in any order, so a wait for one is a wait for all of them and for the LDS reads between.  The
+// token loops therefore go in groups of four: what the next group needs is asked for right behind a wait that has
+// nothing younger in it, and a group's work hides it.  (Left to itself the compiler loads in front of each use: 2000
+// of 3700 cycles of a backward tile were such waits.)
+__device__ __forceinline__ void group_arrived() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);                                    // lgkmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void group_asked() { __builtin_amdgcn_sched_barrier(0); }
 
 // a block of W waves has 64 channels x 4 quads of a tile to load: items per thread
 template <int W> struct ScanItems { static constexpr int N = W >= 4 ? 1 : 4 / W; };
@@ -120,7 +146,7 @@ template <int W> struct ScanItem {
 
 __device__ __forceinline__ float step_size(const Scan& a, float raw) { return a.softplus ? softplus(raw) : raw; }
 
-// B and C as the scan's waves read them: [b][g][token][wave][B0..B3 C0..C3], zeros behind the last state and token.
+// B and C as the scan's waves read them: [b][g][wave][token][B0..B3 C0..C3], zeros behind the last state and token.
 // Threads run along the tokens, so the reads are whole lines.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -139,7 +165,7 @@ bc_prep_kernel(const T* __restrict__ Bm, const T* __restrict__ Cm, float* __rest
         }
         Raw<float, 8> o;
         o.pack(v);
-        o.store(bc + ((bg * Lp + t) * W + w) * 8);
+        o.store(bc + ((bg * W + w) * Lp + t) * 8);
     }
 }
 
@@ -180,7 +206,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) A[s] *= LOG2E;
     const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
-    const f32x8* bc = reinterpret_cast<const f32x8*>(bc0) + (int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave;
+    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
     ScanItem<W> it[NI];
     float bias[NI];
     Quad<T> qd[NI], qx[NI], qz[NI];
@@ -222,18 +248,33 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
         }
         if (n + 1 < t1 - t0) fetch(REV ? tile - 1 : tile + 1);
         __syncthreads();
-        const f32x8* bt = bc + (int64_t)tile * ST * W;
-#pragma unroll 8
-        for (int i = 0; i < ST; ++i) {
-            const int tt = REV ? ST - 1 - i : i;
-            const f32x8 v = bt[tt * W];
-            const float dt = dts[tt][p.lane], u = us[tt][p.lane];
-            sum += dt;
+        BC4 v, vn;
+        float dt[4], u[4], dtn[4], un[4];
+        auto ask = [&](int g) {                                            // the g-th group on the way
+            const int j0 = (REV ? 3 - g : g) * 4;
+            vn.load(bc, (int64_t)tile * ST + j0);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const float decay = __builtin_amdgcn_exp2f(dt * A[s]);
-                if constexpr (REV) h[s] = decay * fmaf(u, v[4 + s], h[s]);
-                else h[s] = fmaf(decay, h[s], u * v[s]);
+            for (int j = 0; j < 4; ++j) { dtn[j] = dts[j0 + j][p.lane]; un[j] = us[j0 + j][p.lane]; }
+        };
+        ask(0);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            group_arrived();
+            v = vn;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; }
+            if (g < 3) ask(g + 1);
+            group_asked();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = REV ? 3 - i : i;
+                sum += dt[j];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const float decay = __builtin_amdgcn_exp2f(dt[j] * A[s]);
+                    if constexpr (REV) h[s] = decay * fmaf(u[j], v.C(j, s), h[s]);
+                    else h[s] = fmaf(decay, h[s], u[j] * v.B(j, s));
+                }
             }
         }
         __syncthreads();
@@ -292,7 +333,7 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
         for (int s = 0; s < 4; ++s)
             h[s] = fmaf(__builtin_amdgcn_exp2f(sum * A[s]), h[s], a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + dr]);
     }
-    const f32x8* bc = reinterpret_cast<const f32x8*>(bc0) + (int64_t)(p.b * a.G + p.g) * a.tiles * ST * W + p.wave;
+    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
     for (int tile = t0; tile < t1; ++tile) {
         const bool full = (int64_t)(tile + 1) * ST <= a.L;
         float x[NI][4], gate[NI][4];
@@ -317,18 +358,32 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
             for (int s = 0; s < 4; ++s)
                 a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + d] = h[s];
         }
-        const f32x8* bt = bc + (int64_t)tile * ST * W;
-#pragma unroll 8
-        for (int i = 0; i < ST; ++i) {
-            const f32x8 v = bt[i * W];
-            const float dt = dts[i][p.lane], u = us[i][p.lane];
-            float y = 0.f;
+        BC4 v, vn;
+        float dt[4], u[4], dtn[4], un[4];
+        auto ask = [&](int g) {                                            // the g-th group on the way
+            vn.load(bc, (int64_t)tile * ST + g * 4);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                h[s] = fmaf(__builtin_amdgcn_exp2f(dt * A[s]), h[s], u * v[s]);
-                y = fmaf(v[4 + s], h[s], y);
+            for (int j = 0; j < 4; ++j) { dtn[j] = dts[g * 4 + j][p.lane]; un[j] = us[g * 4 + j][p.lane]; }
+        };
+        ask(0);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            group_arrived();
+            v = vn;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; }
+            if (g < 3) ask(g + 1);
+            group_asked();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float y = 0.f;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    h[s] = fmaf(__builtin_amdgcn_exp2f(dt[j] * A[s]), h[s], u[j] * v.B(j, s));
+                    y = fmaf(v.C(j, s), h[s], y);
+                }
+                part[p.wave][g * 4 + j][p.lane] = y;
             }
-            part[p.wave][i][p.lane] = y;
         }
         __syncthreads();
 #pragma unroll
@@ -445,74 +500,103 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
             g[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), g[s], a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + dr]);
     }
     const int64_t bg = (int64_t)p.b * a.G + p.g;
-    const f32x8* bc = reinterpret_cast<const f32x8*>(bc0) + bg * a.tiles * ST * W + p.wave;
+    const float* bc = bc0 + (bg * W + p.wave) * a.tiles * ST * 8;
     float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * 2 * W + p.wave) * 64 + p.lane;
     for (int tile = t1 - 1; tile >= t0; --tile) {
         const bool full = (int64_t)(tile + 1) * ST <= a.L;
-        float x[NI][4], dt[NI][4], e[NI][4], raw[NI][4], slope[NI][4];          // slope: dy silu'(z)
+        float x[NI][4], raw[NI][4], slope[NI][4];                               // slope: dy silu'(z)
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw[k], dt[k]);
+            float dt[4];
+            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw[k], dt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[k][i] = qx[k].r.get(i);
-                e[k][i] = it[k].ok ? qy[k].r.get(i) : 0.f;
+                float e = it[k].ok ? qy[k].r.get(i) : 0.f;
                 if constexpr (Z) {
                     const float z = qz[k].r.get(i), q = sigmoid(z);
-                    slope[k][i] = e[k][i] * (q * fmaf(z, 1.0f - q, 1.0f));
-                    e[k][i] *= z * q;
+                    slope[k][i] = e * (q * fmaf(z, 1.0f - q, 1.0f));
+                    e *= z * q;
                 }
                 if (ScanItem<W>::has(k)) {
-                    dts[it[k].q * 4 + i][it[k].r] = dt[k][i];
-                    us[it[k].q * 4 + i][it[k].r] = dt[k][i] * x[k][i];
-                    es[it[k].q * 4 + i][it[k].r] = e[k][i];
+                    dts[it[k].q * 4 + i][it[k].r] = dt[i];
+                    us[it[k].q * 4 + i][it[k].r] = dt[i] * x[k][i];
+                    es[it[k].q * 4 + i][it[k].r] = e;
                 }
             }
         }
         float hs[ST + 1][4], as[ST][4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) hs[0][s] = ok ? hn[s] : 0.f;
-        if (tile > t0) fetch(tile - 1);
         __syncthreads();
-        const f32x8* bt = bc + (int64_t)tile * ST * W;
+        BC4 v, vn;
+        float dt[4], u[4], e[4], dtn[4], un[4], en[4];
+        auto ask = [&](int j0, bool with_e) {                              // the group of tokens j0 .. j0 + 3 on the way
+            vn.load(bc, (int64_t)tile * ST + j0);
 #pragma unroll
-        for (int i = 0; i < ST; ++i) {
-            const f32x8 v = bt[i * W];
-            const float dti = dts[i][p.lane], u = us[i][p.lane];
-            float y = 0.f;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                as[i][s] = __builtin_amdgcn_exp2f(dti * A2[s]);
-                hs[i + 1][s] = fmaf(as[i][s], hs[i][s], u * v[s]);
-                if constexpr (Z) y = fmaf(v[4 + s], hs[i + 1][s], y);
+            for (int j = 0; j < 4; ++j) {
+                dtn[j] = dts[j0 + j][p.lane];
+                un[j] = us[j0 + j][p.lane];
+                if (with_e) en[j] = es[j0 + j][p.lane];
             }
-            if constexpr (Z) part2[p.wave][i][p.lane] = y;
+        };
+        auto take = [&]() {
+            group_arrived();
+            v = vn;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; e[j] = en[j]; }
+        };
+        ask(0, false);
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+            take();
+            if (g4 < 3) ask(g4 * 4 + 4, false);
+            else ask(12, true);
+            group_asked();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = g4 * 4 + j;
+                float y = 0.f;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    as[i][s] = __builtin_amdgcn_exp2f(dt[j] * A2[s]);
+                    hs[i + 1][s] = fmaf(as[i][s], hs[i][s], u[j] * v.B(j, s));
+                    if constexpr (Z) y = fmaf(v.C(j, s), hs[i + 1][s], y);
+                }
+                if constexpr (Z) part2[p.wave][i][p.lane] = y;
+            }
         }
         float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
 #pragma unroll
-        for (int i = ST - 1; i >= 0; --i) {
-            const f32x8 v = bt[i * W];
-            const float dti = dts[i][p.lane], u = us[i][p.lane], ei = es[i][p.lane];
-            float gB = 0.f, gA = 0.f, pr[8];
+        for (int g4 = 3; g4 >= 0; --g4) {
+            take();
+            if (g4 > 0) ask(g4 * 4 - 4, true);
+            if (g4 == 1 && tile > t0) fetch(tile - 1);                     // (half of the states are done with: registers are free)
+            group_asked();
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                g[s] = fmaf(v[4 + s], ei, g[s]);
-                pr[s] = g[s] * u;
-                pr[4 + s] = hs[i + 1][s] * ei;
-                gB = fmaf(g[s], v[s], gB);
-                g[s] *= as[i][s];
-                const float q = g[s] * hs[i][s];
-                gA = fmaf(A[s], q, gA);
-                tA[s] = fmaf(dti, q, tA[s]);
-            }
-            part0[p.wave][i][p.lane] = gB;
-            part1[p.wave][i][p.lane] = gA;
-            if constexpr (!WHOLE) {
+            for (int j = 3; j >= 0; --j) {
+                const int i = g4 * 4 + j;
+                float gB = 0.f, gA = 0.f, pr[8];
 #pragma unroll
-                for (int s = 0; s < 8; ++s) pr[s] = ok ? pr[s] : 0.f;
+                for (int s = 0; s < 4; ++s) {
+                    g[s] = fmaf(v.C(j, s), e[j], g[s]);
+                    pr[s] = g[s] * u[j];
+                    pr[4 + s] = hs[i + 1][s] * e[j];
+                    gB = fmaf(g[s], v.B(j, s), gB);
+                    g[s] *= as[i][s];
+                    const float q = g[s] * hs[i][s];
+                    gA = fmaf(A[s], q, gA);
+                    tA[s] = fmaf(dt[j], q, tA[s]);
+                }
+                part0[p.wave][i][p.lane] = gB;
+                part1[p.wave][i][p.lane] = gA;
+                if constexpr (!WHOLE) {
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) pr[s] = ok ? pr[s] : 0.f;
+                }
+                fold[i & 7] = lanes_fold(pr, p.lane);
+                if ((i & 7) == 0) bco[((int64_t)tile * 2 + (i >> 3)) * W * 64] = tokens_fold(fold, p.lane);
             }
-            fold[i & 7] = lanes_fold(pr, p.lane);
-            if ((i & 7) == 0) bco[((int64_t)tile * 2 + (i >> 3)) * W * 64] = tokens_fold(fold, p.lane);
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) dA[s] += tA[s];
@@ -530,11 +614,12 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                     gB += part0[w][it[k].q * 4 + i][it[k].r];
                     gA += part1[w][it[k].q * 4 + i][it[k].r];
                 }
-                ox[i] = fmaf(gB, dt[k][i], skip[k] * e[k][i]);
+                const float dti = dts[it[k].q * 4 + i][it[k].r], ei = es[it[k].q * 4 + i][it[k].r];
+                ox[i] = fmaf(gB, dti, skip[k] * ei);
                 od[i] = fmaf(gB, x[k][i], gA);
                 if (a.softplus) od[i] *= sigmoid(raw[k][i]);
                 if (full || t + i < a.L) {
-                    dD[k] = fmaf(e[k][i], x[k][i], dD[k]);
+                    dD[k] = fmaf(ei, x[k][i], dD[k]);
                     db[k] += od[i];
                 }
             }

@@ -46,15 +46,8 @@ template <typename T, int K> struct Raw {
 
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(v * LOG2E); }
-// e^v with the product's rounding given back: v log2 e rounded is off by up to |v| 2^-24, and so is the result
-__device__ __forceinline__ float exp_near(float v) {
-    const float t = v * LOG2E;
-    const float low = fmaf(v, 1.9259629911e-8f, fmaf(v, LOG2E, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fabsf(t) < 200.f ? fmaf(e, low * 0.6931471805599453f, e) : e;    // (infinite v: low is no number)
-}
 __device__ __forceinline__ float rcp_fast(float v) { return __builtin_amdgcn_rcpf(v); }     // 1 ulp
 // 1 / (1 + e^-v): e^-v = inf for a very negative v gives 0, as it should
-__device__ __forceinline__ float sigmoid(float v) { return rcp_fast(1.0f + exp_near(-v)); }
+__device__ __forceinline__ float sigmoid(float v) { return rcp_fast(1.0f + exp_fast(-v)); }
 
 }  // namespace rst
