@@ -289,7 +289,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 template <typename T, int W, bool Z>
-__global__ void __launch_bounds__(64 * W)
+__global__ void __launch_bounds__(64 * W, 6)
 scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
     constexpr int NI = ScanItems<W>::N;
     __shared__ float dts[ST][SROW], us[ST][SROW], part[W][ST][SROW];
@@ -786,7 +786,7 @@ static void scan_plan(Scan* a, bool bwd) {
     a->Dg = a->D / a->G;
     a->cb = (int)cdiv(a->Dg, SC);
     a->tiles = (int)cdiv(a->L, ST);
-    const int64_t blocks = (int64_t)a->B * a->G * a->cb, slots = bwd ? 512 : 1024;
+    const int64_t blocks = (int64_t)a->B * a->G * a->cb, slots = bwd ? 512 : 1536;
     const double again = bwd ? 1.2 : 1.6;
     double best = (double)cdiv(blocks, slots) * a->tiles;
     a->per_chunk = a->tiles;
