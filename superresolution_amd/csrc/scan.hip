@@ -76,49 +76,61 @@ struct ScanPlace {
     }
 };
 
-// four tokens of one channel; `full`: the tile ends within the row (the same for the whole block, so no branch)
+// A block's 64 rows of a tensor at a tile: one address for the whole block, and offsets of 32 bits to a thread's channel and
+// tokens (64 L values reach 2^32 bytes at 2^24 tokens, the longest row taken).  left: tokens from the tile's start to the
+// row's end; whether all 16 are there is the same for the whole block.
+struct ScanTile {
+    int64_t at; int left;
+    __device__ __forceinline__ bool full() const { return left >= ST; }
+};
+
+// four tokens of one channel
 template <typename T> struct Quad {
     Raw<T, 4> r;
-    __device__ __forceinline__ void load(const void* tensor, int64_t row, int64_t t, int64_t L, bool full) {
-        const T* p = static_cast<const T*>(tensor) + row;
-        if (full) { r.load(p + t); return; }
+    __device__ __forceinline__ void load(const void* tensor, const ScanTile& tl, uint32_t row, int q) {
+        const char* p = reinterpret_cast<const char*>(static_cast<const T*>(tensor) + tl.at);
+        if (tl.full()) { r.load(reinterpret_cast<const T*>(p + (row + q * 4) * (uint32_t)sizeof(T))); return; }
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = t + i < L ? Store<T>::get(p[t + i]) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+            const int t = q * 4 + i < tl.left ? q * 4 + i : tl.left - 1;
+            const float w = Store<T>::get(*reinterpret_cast<const T*>(p + (row + t) * (uint32_t)sizeof(T)));
+            v[i] = q * 4 + i < tl.left ? w : 0.f;
+        }
         r.pack(v);
     }
-    static __device__ __forceinline__ void put(void* tensor, int64_t row, int64_t t, int64_t L, bool full, bool ok, const float (&v)[4]) {
+    static __device__ __forceinline__ void put(void* tensor, const ScanTile& tl, uint32_t row, int q, bool ok, const float (&v)[4]) {
         if (!ok) return;
-        T* p = static_cast<T*>(tensor) + row;
-        if (full) {
+        char* p = reinterpret_cast<char*>(static_cast<T*>(tensor) + tl.at);
+        if (tl.full()) {
             Raw<T, 4> o;
             o.pack(v);
-            o.store(p + t);
+            o.store(reinterpret_cast<T*>(p + (row + q * 4) * (uint32_t)sizeof(T)));
             return;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (t + i < L) p[t + i] = Store<T>::put(v[i]);
+            if (q * 4 + i < tl.left) *reinterpret_cast<T*>(p + (row + q * 4 + i) * (uint32_t)sizeof(T)) = Store<T>::put(v[i]);
     }
 };
 
-// B and C of four tokens and a wave's four states (scalar registers): token j's B is v[j / 2][8 (j % 2) + s], its C
-// v[j / 2][8 (j % 2) + 4 + s].
+// B and C of K (2 or 4) tokens and a wave's four states, in scalar registers
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-struct BC4 {
-    f32x16 v[2];
+template <int K> struct TokensBC {
+    f32x16 v[K / 2];
     __device__ __forceinline__ void load(const float* __restrict__ bc, int64_t t) {
         const f32x16* p = reinterpret_cast<const f32x16*>(bc + t * 8);
-        v[0] = p[0];
-        v[1] = p[1];
+#pragma unroll
+        for (int i = 0; i < K / 2; ++i) v[i] = p[i];
     }
     __device__ __forceinline__ float B(int j, int s) const { return v[j >> 1][(j & 1) * 8 + s]; }
     __device__ __forceinline__ float C(int j, int s) const { return v[j >> 1][(j & 1) * 8 + 4 + s]; }
 };
 // Scalar loads come back in any order, so a wait for one is a wait for all of them and for the LDS reads between.  The
-// token loops therefore go in groups of four: what the next group needs is asked for right behind a wait that has
-// nothing younger in it, and a group's work hides it.  (Left to itself the compiler loads in front of each use: 2000
-// of 3700 cycles of a backward tile were such waits.)
+// token loops therefore go in groups: what the next group needs is asked for right behind a wait that has nothing
+// younger in it, and a group's work hides it (left to itself the compiler loads in front of each use: backward 1108
+// against 887 us).  Four tokens a group; two backward, whose token is four times the work and whose scalar registers
+// would spill to lanes of vector registers.
 __device__ __forceinline__ void group_arrived() {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xC07F);                                    // lgkmcnt(0)
@@ -129,9 +141,9 @@ __device__ __forceinline__ void group_asked() { __builtin_amdgcn_sched_barrier(0
 // a block of W waves has 64 channels x 4 quads of a tile to load: items per thread
 template <int W> struct ScanItems { static constexpr int N = W >= 4 ? 1 : 4 / W; };
 
-// the channel, quad and address of one of a thread's items; a thread without one reads channel 0 and writes nothing
+// the channel, quad and row of one of a thread's items; a thread without one reads channel 0 and writes nothing
 template <int W> struct ScanItem {
-    int r, q, d; bool ok; int64_t row;
+    int r, q, d; bool ok; uint32_t row;
     __device__ __forceinline__ ScanItem() {}
     __device__ __forceinline__ void set(const Scan& a, const ScanPlace& p, int k) {
         const int i = threadIdx.x + k * 64 * W;
@@ -139,10 +151,14 @@ template <int W> struct ScanItem {
         q = i & 3;
         d = p.g * a.Dg + p.cb * SC + r;
         ok = i < 256 && p.cb * SC + r < a.Dg;
-        row = ((int64_t)p.b * a.D + (ok ? d : 0)) * a.L;
+        row = ok ? (uint32_t)r * (uint32_t)a.L : 0u;
     }
     static __device__ __forceinline__ bool has(int k) { return W <= 4 || threadIdx.x < 256; }
 };
+__device__ __forceinline__ ScanTile scan_tile(const Scan& a, const ScanPlace& p, int tile) {
+    const int64_t t = (int64_t)tile * ST;
+    return {((int64_t)p.b * a.D + p.g * a.Dg + p.cb * SC) * a.L + t, (int)(a.L - t < ST ? a.L - t : ST)};
+}
 
 __device__ __forceinline__ float step_size(const Scan& a, float raw) { return a.softplus ? softplus(raw) : raw; }
 
@@ -177,13 +193,13 @@ __device__ __forceinline__ void load_rates(const Scan& a, int d, bool ok, int wa
 
 // dt of four tokens: zero where there is no channel or token, so that nothing there moves a state
 template <typename T>
-__device__ __forceinline__ void step_sizes(const Scan& a, const Quad<T>& q, float bias, int64_t t, bool full, bool ok, float (&raw)[4],
-                                           float (&dt)[4]) {
+__device__ __forceinline__ void step_sizes(const Scan& a, const Quad<T>& qd, float bias, const ScanTile& tl, int q, bool ok,
+                                           float (&raw)[4], float (&dt)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        raw[i] = q.r.get(i) + bias;
-        const float v = step_size(a, raw[i]);
-        dt[i] = ok && (full || t + i < a.L) ? v : 0.f;
+        raw[i] = qd.r.get(i) + bias;
+        dt[i] = step_size(a, raw[i]);
+        if (!ok || q * 4 + i >= tl.left) dt[i] = 0.f;
     }
 }
 template <typename T>
@@ -211,13 +227,12 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     float bias[NI];
     Quad<T> qd[NI], qx[NI], qz[NI];
     auto fetch = [&](int tile) {
-        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        const ScanTile tl = scan_tile(a, p, tile);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
-            qd[k].load(a.delta, it[k].row, t, a.L, full);
-            qx[k].load(REV ? a.dy : a.x, it[k].row, t, a.L, full);
-            if constexpr (REV && Z) qz[k].load(a.z, it[k].row, t, a.L, full);
+            qd[k].load(a.delta, tl, it[k].row, it[k].q);
+            qx[k].load(REV ? a.dy : a.x, tl, it[k].row, it[k].q);
+            if constexpr (REV && Z) qz[k].load(a.z, tl, it[k].row, it[k].q);
         }
     };
 #pragma unroll
@@ -228,11 +243,11 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     fetch(REV ? t1 - 1 : t0);
     for (int n = 0; n < t1 - t0; ++n) {
         const int tile = REV ? t1 - 1 - n : t0 + n;
-        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        const ScanTile tl = scan_tile(a, p, tile);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             float raw[4], dt[4];
-            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw, dt);
+            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, raw, dt);
             if (ScanItem<W>::has(k)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -248,7 +263,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
         }
         if (n + 1 < t1 - t0) fetch(REV ? tile - 1 : tile + 1);
         __syncthreads();
-        BC4 v, vn;
+        TokensBC<4> v, vn;
         float dt[4], u[4], dtn[4], un[4];
         auto ask = [&](int g) {                                            // the g-th group on the way
             const int j0 = (REV ? 3 - g : g) * 4;
@@ -301,13 +316,12 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
     float bias[NI], skip[NI];
     Quad<T> qd[NI], qx[NI], qz[NI];
     auto fetch = [&](int tile) {
-        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        const ScanTile tl = scan_tile(a, p, tile);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
-            qd[k].load(a.delta, it[k].row, t, a.L, full);
-            qx[k].load(a.x, it[k].row, t, a.L, full);
-            if constexpr (Z) qz[k].load(a.z, it[k].row, t, a.L, full);
+            qd[k].load(a.delta, tl, it[k].row, it[k].q);
+            qx[k].load(a.x, tl, it[k].row, it[k].q);
+            if constexpr (Z) qz[k].load(a.z, tl, it[k].row, it[k].q);
         }
     };
 #pragma unroll
@@ -335,12 +349,12 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
     }
     const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
     for (int tile = t0; tile < t1; ++tile) {
-        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        const ScanTile tl = scan_tile(a, p, tile);
         float x[NI][4], gate[NI][4];
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             float raw[4], dt[4];
-            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw, dt);
+            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, raw, dt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[k][i] = qx[k].r.get(i);
@@ -356,9 +370,9 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
         if (a.ckpt && ok) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
-                a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + d] = h[s];
+                (a.ckpt + (((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D)[(uint32_t)d] = h[s];
         }
-        BC4 v, vn;
+        TokensBC<4> v, vn;
         float dt[4], u[4], dtn[4], un[4];
         auto ask = [&](int g) {                                            // the g-th group on the way
             vn.load(bc, (int64_t)tile * ST + g * 4);
@@ -397,7 +411,7 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
                 for (int w = 0; w < W; ++w) y[i] += part[w][it[k].q * 4 + i][it[k].r];
                 if constexpr (Z) y[i] *= gate[k][i];
             }
-            Quad<T>::put(a.y, it[k].row, (int64_t)tile * ST + it[k].q * 4, a.L, full, it[k].ok, y);
+            Quad<T>::put(a.y, tl, it[k].row, it[k].q, it[k].ok, y);
         }
     }
     if (a.last && ok && t1 == a.tiles) {
@@ -471,17 +485,16 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
     Quad<T> qd[NI], qx[NI], qy[NI], qz[NI];
     float hn[4];
     auto fetch = [&](int tile) {
-        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        const ScanTile tl = scan_tile(a, p, tile);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
-            qd[k].load(a.delta, it[k].row, t, a.L, full);
-            qx[k].load(a.x, it[k].row, t, a.L, full);
-            qy[k].load(a.dy, it[k].row, t, a.L, full);
-            if constexpr (Z) qz[k].load(a.z, it[k].row, t, a.L, full);
+            qd[k].load(a.delta, tl, it[k].row, it[k].q);
+            qx[k].load(a.x, tl, it[k].row, it[k].q);
+            qy[k].load(a.dy, tl, it[k].row, it[k].q);
+            if constexpr (Z) qz[k].load(a.z, tl, it[k].row, it[k].q);
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) hn[s] = a.ckpt[(((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D + dr];
+        for (int s = 0; s < 4; ++s) hn[s] = (a.ckpt + (((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D)[(uint32_t)dr];
     };
     fetch(t1 - 1);
     float A[4], A2[4], g[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
@@ -501,14 +514,14 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
     }
     const int64_t bg = (int64_t)p.b * a.G + p.g;
     const float* bc = bc0 + (bg * W + p.wave) * a.tiles * ST * 8;
-    float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * 2 * W + p.wave) * 64 + p.lane;
+    float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * 2 * W + p.wave) * 64;
     for (int tile = t1 - 1; tile >= t0; --tile) {
-        const bool full = (int64_t)(tile + 1) * ST <= a.L;
+        const ScanTile tl = scan_tile(a, p, tile);
         float x[NI][4], raw[NI][4], slope[NI][4];                               // slope: dy silu'(z)
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             float dt[4];
-            step_sizes<T>(a, qd[k], bias[k], (int64_t)tile * ST + it[k].q * 4, full, it[k].ok, raw[k], dt);
+            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, raw[k], dt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[k][i] = qx[k].r.get(i);
@@ -529,12 +542,13 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
 #pragma unroll
         for (int s = 0; s < 4; ++s) hs[0][s] = ok ? hn[s] : 0.f;
         __syncthreads();
-        BC4 v, vn;
-        float dt[4], u[4], e[4], dtn[4], un[4], en[4];
-        auto ask = [&](int j0, bool with_e) {                              // the group of tokens j0 .. j0 + 3 on the way
-            vn.load(bc, (int64_t)tile * ST + j0);
+        const float* bct = bc + (int64_t)tile * ST * 8;
+        TokensBC<2> v, vn;
+        float dt[2], u[2], e[2], dtn[2], un[2], en[2];
+        auto ask = [&](int j0, bool with_e) {                              // tokens j0 and j0 + 1 on the way
+            vn.load(bct, j0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 dtn[j] = dts[j0 + j][p.lane];
                 un[j] = us[j0 + j][p.lane];
                 if (with_e) en[j] = es[j0 + j][p.lane];
@@ -544,18 +558,22 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
             group_arrived();
             v = vn;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; e[j] = en[j]; }
+            for (int j = 0; j < 2; ++j) { dt[j] = dtn[j]; u[j] = un[j]; e[j] = en[j]; }
         };
         ask(0, false);
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
+        for (int i0 = 0; i0 < ST; i0 += 2) {
             take();
-            if (g4 < 3) ask(g4 * 4 + 4, false);
-            else ask(12, true);
+            if (i0 + 2 < ST) ask(i0 + 2, false);
+            else {
+                // (the way back reads B and C again: the compiler would rather keep all of them, in lanes of vector registers)
+                
+                ask(ST - 2, true);
+            }
             group_asked();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = g4 * 4 + j;
+            for (int j = 0; j < 2; ++j) {
+                const int i = i0 + j;
                 float y = 0.f;
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
@@ -568,14 +586,14 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
         }
         float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
 #pragma unroll
-        for (int g4 = 3; g4 >= 0; --g4) {
+        for (int i0 = ST - 2; i0 >= 0; i0 -= 2) {
             take();
-            if (g4 > 0) ask(g4 * 4 - 4, true);
-            if (g4 == 1 && tile > t0) fetch(tile - 1);                     // (half of the states are done with: registers are free)
+            if (i0 > 0) ask(i0 - 2, true);
+            if (i0 == ST / 2 - 2 && tile > t0) fetch(tile - 1);            // (half of the states are done with: registers are free)
             group_asked();
 #pragma unroll
-            for (int j = 3; j >= 0; --j) {
-                const int i = g4 * 4 + j;
+            for (int j = 1; j >= 0; --j) {
+                const int i = i0 + j;
                 float gB = 0.f, gA = 0.f, pr[8];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
@@ -595,7 +613,7 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                     for (int s = 0; s < 8; ++s) pr[s] = ok ? pr[s] : 0.f;
                 }
                 fold[i & 7] = lanes_fold(pr, p.lane);
-                if ((i & 7) == 0) bco[((int64_t)tile * 2 + (i >> 3)) * W * 64] = tokens_fold(fold, p.lane);
+                if ((i & 7) == 0) (bco + ((int64_t)tile * 2 + (i >> 3)) * W * 64)[(uint32_t)p.lane] = tokens_fold(fold, p.lane);
             }
         }
 #pragma unroll
@@ -604,7 +622,6 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             if (!ScanItem<W>::has(k)) continue;
-            const int64_t t = (int64_t)tile * ST + it[k].q * 4;
             float ox[4], od[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -618,13 +635,11 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                 ox[i] = fmaf(gB, dti, skip[k] * ei);
                 od[i] = fmaf(gB, x[k][i], gA);
                 if (a.softplus) od[i] *= sigmoid(raw[k][i]);
-                if (full || t + i < a.L) {
-                    dD[k] = fmaf(ei, x[k][i], dD[k]);
-                    db[k] += od[i];
-                }
+                dD[k] = fmaf(ei, x[k][i], dD[k]);
+                if (it[k].q * 4 + i < tl.left) db[k] += od[i];              // (behind the row g is the last state's gradient)
             }
-            Quad<T>::put(a.dx, it[k].row, t, a.L, full, it[k].ok, ox);
-            Quad<T>::put(a.ddelta, it[k].row, t, a.L, full, it[k].ok, od);
+            Quad<T>::put(a.dx, tl, it[k].row, it[k].q, it[k].ok, ox);
+            Quad<T>::put(a.ddelta, tl, it[k].row, it[k].q, it[k].ok, od);
             if constexpr (Z) {
                 float oz[4];
 #pragma unroll
@@ -634,7 +649,7 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                     for (int w = 0; w < W; ++w) y += part2[w][it[k].q * 4 + i][it[k].r];
                     oz[i] = slope[k][i] * y;
                 }
-                Quad<T>::put(a.dz, it[k].row, t, a.L, full, it[k].ok, oz);
+                Quad<T>::put(a.dz, tl, it[k].row, it[k].q, it[k].ok, oz);
             }
         }
         __syncthreads();
@@ -804,7 +819,7 @@ static int scan_check(const char* what, const rst_scan_desc* s) {
     RST_REQUIRE(s->B > 0 && s->D > 0 && s->L > 0, "%s: empty shape B=%d D=%d L=%lld", what, s->B, s->D, (long long)s->L);
     RST_REQUIRE(s->G > 0 && s->D % s->G == 0, "%s: D=%d not divisible by groups=%d", what, s->D, s->G);
     RST_REQUIRE(s->N > 0 && s->N <= 32, "%s: N=%d states (1 to 32)", what, s->N);
-    RST_REQUIRE(s->L <= (1ll << 31) && (int64_t)s->B * s->D <= (1ll << 30) && (int64_t)s->B * s->G <= 65535,
+    RST_REQUIRE(s->L <= (1ll << 24) && (int64_t)s->B * s->D <= (1ll << 30) && (int64_t)s->B * s->G <= 65535,
                 "%s: shape out of range B=%d D=%d G=%d L=%lld", what, s->B, s->D, s->G, (long long)s->L);
     return RST_OK;
 }
