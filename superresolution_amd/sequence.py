@@ -16,11 +16,9 @@ leaves without a live eager graph (capture a function that calls ``torch.autogra
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import ScanDesc, ScanGrads, ScanInputs, check
@@ -65,13 +63,28 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _on(t: torch.Tensor):
-    """The inputs' device made current (nothing where it is)."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+# (current_stream() and current_device() build objects and look the device up: 2 us a call, 10 us from the autograd thread,
+# as much as the smallest kernels)
+_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _call(name: str, t: torch.Tensor, *args) -> None:
+    """An entry point of the library on `t`'s device and that device's current stream (the last argument)."""
+    index = t.device.index
+    fn = getattr(_lib.load(), name)
+    if index == _device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status, name)
+
+
+def _first_order_only(name: str) -> None:
+    if torch.is_grad_enabled():                  # only under create_graph=True
+        raise RuntimeError(f"{name}: gradients are first-order only")
 
 
 def _scratch(nbytes: int, t: torch.Tensor) -> torch.Tensor:
@@ -79,7 +92,11 @@ def _scratch(nbytes: int, t: torch.Tensor) -> torch.Tensor:
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _next_state(state: torch.Tensor, state_out: Optional[torch.Tensor], name: str) -> torch.Tensor:
@@ -100,12 +117,10 @@ def _next_state(state: torch.Tensor, state_out: Optional[torch.Tensor], name: st
 # layer norm of token rows
 # ----------------------------------------------------------------------------
 def _norm_forward(x, weight, bias, eps):
-    lib = _lib.load()
     y = torch.empty_like(x)
-    if x.numel():
-        with _on(x):
-            check(lib.rst_rows_norm_fwd(_ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(bias), _ptr(y), x.numel() // x.shape[-1],
-                                        x.shape[-1], eps, _stream(x)), "rst_rows_norm_fwd")
+    n, C = x.numel(), x.shape[-1]
+    if n:
+        _call("rst_rows_norm_fwd", x, x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), _ptr(bias), y.data_ptr(), n // C, C, eps)
     return y
 
 
@@ -117,9 +132,8 @@ class _LayerNormFn(torch.autograd.Function):
         return _norm_forward(x, weight, bias, eps)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        lib = _lib.load()
+        _first_order_only("layernorm")
         x, weight = ctx.saved_tensors
         if x.numel() == 0:
             return torch.zeros_like(x), torch.zeros_like(weight), torch.zeros_like(weight) if ctx.with_bias else None, None
@@ -127,10 +141,10 @@ class _LayerNormFn(torch.autograd.Function):
         dx, dw = torch.empty_like(x), torch.empty_like(weight)
         db = torch.empty_like(weight) if ctx.with_bias else None
         rows, C = x.numel() // x.shape[-1], x.shape[-1]
-        with _on(x):
-            ws = _scratch(lib.rst_rows_norm_bwd_workspace_bytes(rows, C), x)
-            check(lib.rst_rows_norm_bwd(_ptr(x), _DTYPES[x.dtype], _ptr(weight), int(ctx.with_bias), _ptr(dy), _ptr(dx), _ptr(dw),
-                                        _ptr(db), rows, C, ctx.eps, _ptr(ws), ws.numel(), _stream(x)), "rst_rows_norm_bwd")
+        nb = _lib.load().rst_rows_norm_bwd_workspace_bytes(rows, C)
+        ws = _scratch(nb, x)
+        _call("rst_rows_norm_bwd", x, x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), int(ctx.with_bias), dy.data_ptr(),
+              dx.data_ptr(), dw.data_ptr(), _ptr(db), rows, C, ctx.eps, ws.data_ptr(), nb)
         return dx, dw, db, None
 
 
@@ -156,15 +170,13 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
 # short causal convolution
 # ----------------------------------------------------------------------------
 def _conv_forward(x, weight, bias, state, silu, want_state):
-    lib = _lib.load()
     B, D, L = x.shape
     W = weight.shape[1]
     y = torch.empty_like(x)
     end = torch.empty((B, D, W - 1), dtype=x.dtype, device=x.device) if want_state else None
     if x.numel():
-        with _on(x):
-            check(lib.rst_causal_conv1d_fwd(_ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(bias), _ptr(state), _ptr(y), _ptr(end),
-                                            B, D, L, W, int(silu), _stream(x)), "rst_causal_conv1d_fwd")
+        _call("rst_causal_conv1d_fwd", x, x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), _ptr(bias), _ptr(state), y.data_ptr(),
+              _ptr(end), B, D, L, W, int(silu))
     elif want_state:
         end.zero_() if state is None else end.copy_(state)
     return y, end
@@ -180,9 +192,8 @@ class _CausalConvFn(torch.autograd.Function):
         return (y, end) if want_state else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dend=None):
-        lib = _lib.load()
+        _first_order_only("causal_conv1d")
         x, weight, bias, state = ctx.saved_tensors
         B, D, L = x.shape
         W = weight.shape[1]
@@ -196,11 +207,10 @@ class _CausalConvFn(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else _act(dy, "causal_conv1d dy", x)
         dx, dw = torch.empty_like(x), torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
-        with _on(x):
-            ws = _scratch(lib.rst_causal_conv1d_bwd_workspace_bytes(B, D, L), x)
-            check(lib.rst_causal_conv1d_bwd(_ptr(x), _DTYPES[x.dtype], _ptr(weight), _ptr(bias), _ptr(state), _ptr(dy), _ptr(dend),
-                                            _ptr(dx), _ptr(dw), _ptr(db), _ptr(dstate), B, D, L, W, int(ctx.silu), _ptr(ws),
-                                            ws.numel(), _stream(x)), "rst_causal_conv1d_bwd")
+        nb = _lib.load().rst_causal_conv1d_bwd_workspace_bytes(B, D, L)
+        ws = _scratch(nb, x)
+        _call("rst_causal_conv1d_bwd", x, x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), _ptr(bias), _ptr(state), dy.data_ptr(),
+              _ptr(dend), dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(dstate), B, D, L, W, int(ctx.silu), ws.data_ptr(), nb)
         return dx, dw, db, dstate, None, None
 
 
@@ -248,12 +258,10 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     B, D, W = x.shape[0], x.shape[1], weight.shape[1]
     _shape(state, "causal_conv1d_update state", (B, D, W - 1))
     state, out = _act(state, "causal_conv1d_update state", x), _next_state(state, state_out, "causal_conv1d_update")
-    lib = _lib.load()
     y = torch.empty_like(x)
     if x.numel():
-        with _on(x):
-            check(lib.rst_causal_conv1d_update(_ptr(x), _DTYPES[x.dtype], _ptr(state), _ptr(out), _ptr(weight), _ptr(bias), _ptr(y), B, D,
-                                               W, int(activation == "silu"), _stream(x)), "rst_causal_conv1d_update")
+        _call("rst_causal_conv1d_update", x, x.data_ptr(), _DTYPES[x.dtype], state.data_ptr(), out.data_ptr(), weight.data_ptr(),
+              _ptr(bias), y.data_ptr(), B, D, W, int(activation == "silu"))
     return y
 
 
@@ -277,12 +285,11 @@ def _scan_forward(x, delta, A, B, C, D, z, delta_bias, h0, softplus, want_last, 
     if x.numel():
         desc, ins = _scan_desc(x, A, B, softplus), _scan_inputs(x, delta, A, B, C, D, z, delta_bias)
         ref = ctypes.byref(desc)
-        with _on(x):
-            if keep:
-                saved = _scratch(lib.rst_scan_saved_bytes(ref), x)
-            ws = _scratch(lib.rst_scan_workspace_bytes(ref), x)
-            check(lib.rst_scan_fwd(ref, ctypes.byref(ins), _ptr(h0), _ptr(y), _ptr(last), _ptr(saved), _ptr(ws), ws.numel(),
-                                   _stream(x)), "rst_scan_fwd")
+        if keep:
+            saved = _scratch(lib.rst_scan_saved_bytes(ref), x)
+        nb = lib.rst_scan_workspace_bytes(ref)
+        ws = _scratch(nb, x)
+        _call("rst_scan_fwd", x, ref, ctypes.byref(ins), _ptr(h0), y.data_ptr(), _ptr(last), _ptr(saved), ws.data_ptr(), nb)
     elif want_last:
         last.zero_() if h0 is None else last.copy_(h0)
     return y, last, saved
@@ -298,9 +305,8 @@ class _ScanFn(torch.autograd.Function):
         return (y, last) if want_last else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast=None):
-        lib = _lib.load()
+        _first_order_only("selective_scan")
         *ins, saved = ctx.saved_tensors
         x, delta, A, B, C, D, z, delta_bias = ins
         dlast = _par(dlast, "selective_scan last state's gradient", x)
@@ -313,10 +319,10 @@ class _ScanFn(torch.autograd.Function):
         grads = [None if t is None else torch.empty_like(t) for t in ins]
         desc, inputs, outs = _scan_desc(x, A, B, ctx.softplus), _scan_inputs(*ins), ScanGrads(*[_ptr(g) for g in grads])
         ref = ctypes.byref(desc)
-        with _on(x):
-            ws = _scratch(lib.rst_scan_bwd_workspace_bytes(ref), x)
-            check(lib.rst_scan_bwd(ref, ctypes.byref(inputs), _ptr(saved), _ptr(dy), _ptr(dlast), ctypes.byref(outs), _ptr(dh0),
-                                   _ptr(ws), ws.numel(), _stream(x)), "rst_scan_bwd")
+        nb = _lib.load().rst_scan_bwd_workspace_bytes(ref)
+        ws = _scratch(nb, x)
+        _call("rst_scan_bwd", x, ref, ctypes.byref(inputs), saved.data_ptr(), dy.data_ptr(), _ptr(dlast), ctypes.byref(outs), _ptr(dh0),
+              ws.data_ptr(), nb)
         return tuple(grads) + (dh0, None, None)
 
 
@@ -384,11 +390,8 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     x, delta, A, B, C, D, z, delta_bias = _scan_args("selective_scan_update", x, delta, A, B, C, D, z, delta_bias)
     _shape(state, "selective_scan_update state", (x.shape[0], x.shape[1], A.shape[1]))
     state, out = _par(state, "selective_scan_update state", x), _next_state(state, state_out, "selective_scan_update")
-    lib = _lib.load()
     y = torch.empty_like(x)
     if x.numel():
         desc, ins = _scan_desc(x, A, B, delta_softplus), _scan_inputs(x, delta, A, B, C, D, z, delta_bias)
-        with _on(x):
-            check(lib.rst_scan_update(ctypes.byref(desc), ctypes.byref(ins), _ptr(state), _ptr(out), _ptr(y), _stream(x)),
-                  "rst_scan_update")
+        _call("rst_scan_update", x, ctypes.byref(desc), ctypes.byref(ins), state.data_ptr(), out.data_ptr(), y.data_ptr())
     return y
