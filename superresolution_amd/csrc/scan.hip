@@ -302,6 +302,55 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     }
 }
 
+// ---- the chunks' own states, one behind the other: cst[c] becomes the state that chunk c starts from (REV: the
+// state's gradient behind it).  A block has 64 channels and one state; its 16 waves take 16 runs of chunks side by side,
+// chain the runs through LDS and walk their run again.  (Chained in front of every chunk by the scan's own blocks, the
+// states are read as often as there are chunks: 503 MB from the caches for 256 chunks of 192 channels, 45 us instead of 20.)
+template <bool REV>
+__global__ void __launch_bounds__(1024)
+scan_chain_kernel(const Scan a, int states) {
+    __shared__ float sums[16][64], own[16][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+    const int d = blockIdx.x * 64 + lane, n = blockIdx.y, b = blockIdx.z;
+    const bool ok = d < a.D;
+    const int dr = ok ? d : 0;
+    const float A = n < a.N ? a.A[(int64_t)dr * a.N + n] * LOG2E : 0.f;
+    const int per = (a.nchunk + 15) / 16, c0 = run * per, c1 = c0 + per < a.nchunk ? c0 + per : a.nchunk;
+    float* st = a.cst + ((int64_t)b * a.nchunk * states + n) * a.D;        // chunk c: + c states D
+    const float* dt = a.cdt + (int64_t)b * a.nchunk * a.D;
+    auto at = [&](int c) { return REV ? a.nchunk - 1 - c : c; };           // the c-th chunk on the way
+    float sum = 0.f, h = 0.f;
+#pragma unroll 4
+    for (int c = c0; c < c1; ++c) {
+        // (the last chunk on the way has nothing behind it and left no state)
+        const float t = c < a.nchunk - 1 ? dt[(int64_t)at(c) * a.D + dr] : 0.f;
+        const float v = c < a.nchunk - 1 ? st[(int64_t)at(c) * states * a.D + dr] : 0.f;
+        sum += t;
+        h = fmaf(__builtin_amdgcn_exp2f(t * A), h, v);
+    }
+    sums[run][lane] = sum;
+    own[run][lane] = h;
+    __syncthreads();
+    const float* first = REV ? a.dlast : a.h0;
+    h = first && n < a.N ? first[((int64_t)b * a.D + dr) * a.N + n] : 0.f;
+    for (int r = 0; r < run; ++r) h = fmaf(__builtin_amdgcn_exp2f(sums[r][lane] * A), h, own[r][lane]);
+    if (!ok) return;
+#pragma unroll 4
+    for (int c = c0; c < c1; ++c) {
+        const float t = c < a.nchunk - 1 ? dt[(int64_t)at(c) * a.D + d] : 0.f;
+        const float v = c < a.nchunk - 1 ? st[(int64_t)at(c) * states * a.D + d] : 0.f;
+        st[(int64_t)at(c) * states * a.D + d] = h;
+        h = fmaf(__builtin_amdgcn_exp2f(t * A), h, v);
+    }
+}
+// what a block starts from: the chained state of its chunk, or the call's own
+template <int W>
+__device__ __forceinline__ float start_state(const Scan& a, const ScanPlace& p, int d, bool ok, int s, const float* first) {
+    if (!ok) return 0.f;
+    if (a.nchunk > 1) return (a.cst + (((int64_t)p.b * a.nchunk + p.chunk) * 4 * W + p.wave * 4 + s) * a.D)[(uint32_t)d];
+    return first && p.wave * 4 + s < a.N ? first[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, 6)
@@ -336,16 +385,7 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         A[s] *= LOG2E;
-        h[s] = a.h0 && ok && p.wave * 4 + s < a.N ? a.h0[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
-    }
-    const int dr = ok ? d : 0;
-#pragma unroll 4
-    for (int c = 0; c < p.chunk; ++c) {
-        const int64_t ci = (int64_t)p.b * a.nchunk + c;
-        const float sum = a.cdt[ci * a.D + dr];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            h[s] = fmaf(__builtin_amdgcn_exp2f(sum * A[s]), h[s], a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + dr]);
+        h[s] = start_state<W>(a, p, d, ok, s, a.h0);
     }
     const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
     for (int tile = t0; tile < t1; ++tile) {
@@ -502,15 +542,7 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         A2[s] = A[s] * LOG2E;
-        g[s] = a.dlast && ok && p.wave * 4 + s < a.N ? a.dlast[((int64_t)p.b * a.D + d) * a.N + p.wave * 4 + s] : 0.f;
-    }
-#pragma unroll 4
-    for (int c = a.nchunk - 1; c > p.chunk; --c) {
-        const int64_t ci = (int64_t)p.b * a.nchunk + c;
-        const float sum = a.cdt[ci * a.D + dr];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            g[s] = fmaf(__builtin_amdgcn_exp2f(sum * A2[s]), g[s], a.cst[(ci * 4 * W + p.wave * 4 + s) * a.D + dr]);
+        g[s] = start_state<W>(a, p, d, ok, s, a.dlast);
     }
     const int64_t bg = (int64_t)p.b * a.G + p.g;
     const float* bc = bc0 + (bg * W + p.wave) * a.tiles * ST * 8;
@@ -795,19 +827,19 @@ static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
 
 // How many chunks a row is cut into.  The chip holds 1024 blocks of the forward kernel (four to a compute unit) or 512 of
 // the backward kernel (two); more run in rounds, so 528 blocks take as long as 1024.  Chunks cost the pass over the
-// chunks' own states, 0.6 of the forward kernel's time and 0.2 of the backward's, and a few steps of a chain per chunk before
-// a block.  The number with the least rounds x tiles is taken, chunks of at least four tiles.
+// chunks' own states, 0.6 of the forward kernel's time and 0.2 of the backward's, and a block costs about half a tile beside
+// its tiles.  The number with the least rounds x tiles is taken, chunks of at least four tiles.
 static void scan_plan(Scan* a, bool bwd) {
     a->Dg = a->D / a->G;
     a->cb = (int)cdiv(a->Dg, SC);
     a->tiles = (int)cdiv(a->L, ST);
     const int64_t blocks = (int64_t)a->B * a->G * a->cb, slots = bwd ? 512 : 1536;
     const double again = bwd ? 1.2 : 1.6;
-    double best = (double)cdiv(blocks, slots) * a->tiles;
+    double best = (double)cdiv(blocks, slots) * (a->tiles + 0.5);
     a->per_chunk = a->tiles;
-    for (int64_t n = 2; n <= a->tiles / 4 && n <= 256 && blocks * n <= 4 * slots; ++n) {
+    for (int64_t n = 2; n <= a->tiles / 4 && n <= 1024 && blocks * n <= 4 * slots; ++n) {
         const int64_t per = cdiv(a->tiles, n), real = cdiv(a->tiles, per);
-        const double cost = (double)cdiv(blocks * real, slots) * per * again + 0.05 * real;
+        const double cost = (double)cdiv(blocks * real, slots) * (per + 0.5) * again + 3.0;
         if (cost < best) { best = cost; a->per_chunk = (int)per; }
     }
     a->nchunk = (int)cdiv(a->tiles, a->per_chunk);
@@ -871,6 +903,8 @@ static int scan_fwd_t(const Scan& a, hipStream_t st) {
     if (a.nchunk > 1) {
         hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
         RST_LAUNCH_CHECK();
+        hipLaunchKernelGGL((scan_chain_kernel<false>), dim3((unsigned)cdiv(a.D, 64), 4 * W, a.B), dim3(1024), 0, st, a, 4 * W);
+        RST_LAUNCH_CHECK();
     }
     hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a, a.bc);
     RST_LAUNCH_CHECK();
@@ -886,6 +920,8 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
         hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        RST_LAUNCH_CHECK();
+        hipLaunchKernelGGL((scan_chain_kernel<true>), dim3((unsigned)cdiv(a.D, 64), 4 * W, a.B), dim3(1024), 0, st, a, 4 * W);
         RST_LAUNCH_CHECK();
     }
     const size_t lds = (size_t)(3 + (Z ? 3 : 2) * W) * ST * SROW * sizeof(float);
