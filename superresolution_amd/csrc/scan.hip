@@ -318,15 +318,23 @@ scan_chain_kernel(const Scan a, int states) {
     const int per = (a.nchunk + 15) / 16, c0 = run * per, c1 = c0 + per < a.nchunk ? c0 + per : a.nchunk;
     float* st = a.cst + ((int64_t)b * a.nchunk * states + n) * a.D;        // chunk c: + c states D
     const float* dt = a.cdt + (int64_t)b * a.nchunk * a.D;
-    auto at = [&](int c) { return REV ? a.nchunk - 1 - c : c; };           // the c-th chunk on the way
-    float sum = 0.f, h = 0.f;
-#pragma unroll 4
-    for (int c = c0; c < c1; ++c) {
-        // (the last chunk on the way has nothing behind it and left no state)
-        const float t = c < a.nchunk - 1 ? dt[(int64_t)at(c) * a.D + dr] : 0.f;
-        const float v = c < a.nchunk - 1 ? st[(int64_t)at(c) * states * a.D + dr] : 0.f;
-        sum += t;
-        h = fmaf(__builtin_amdgcn_exp2f(t * A), h, v);
+    // chunk c on the way; the last one has nothing behind it and left no state
+    auto read = [&](int c, float& t, float& v) {
+        const bool in = c < c1 && c < a.nchunk - 1;
+        const int64_t k = REV ? a.nchunk - 1 - (in ? c : 0) : (in ? c : 0);
+        t = dt[k * a.D + dr];
+        v = st[k * states * a.D + dr];
+        if (!in) { t = 0.f; v = 0.f; }
+    };
+    float sum = 0.f, h = 0.f, t[8], v[8];
+    for (int c = c0; c < c1; c += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) read(c + j, t[j], v[j]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sum += t[j];
+            h = fmaf(__builtin_amdgcn_exp2f(t[j] * A), h, v[j]);
+        }
     }
     sums[run][lane] = sum;
     own[run][lane] = h;
@@ -334,13 +342,18 @@ scan_chain_kernel(const Scan a, int states) {
     const float* first = REV ? a.dlast : a.h0;
     h = first && n < a.N ? first[((int64_t)b * a.D + dr) * a.N + n] : 0.f;
     for (int r = 0; r < run; ++r) h = fmaf(__builtin_amdgcn_exp2f(sums[r][lane] * A), h, own[r][lane]);
-    if (!ok) return;
-#pragma unroll 4
-    for (int c = c0; c < c1; ++c) {
-        const float t = c < a.nchunk - 1 ? dt[(int64_t)at(c) * a.D + d] : 0.f;
-        const float v = c < a.nchunk - 1 ? st[(int64_t)at(c) * states * a.D + d] : 0.f;
-        st[(int64_t)at(c) * states * a.D + d] = h;
-        h = fmaf(__builtin_amdgcn_exp2f(t * A), h, v);
+    for (int c = c0; c < c1; c += 8) {
+        if (c1 - c0 > 8) {                                                 // (a run of at most eight is still in registers)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) read(c + j, t[j], v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c + j < c1) {
+                const int64_t k = REV ? a.nchunk - 1 - (c + j) : c + j;
+                if (ok) st[k * states * a.D + d] = h;
+                h = fmaf(__builtin_amdgcn_exp2f(t[j] * A), h, v[j]);
+            }
     }
 }
 // what a block starts from: the chained state of its chunk, or the call's own
@@ -717,48 +730,50 @@ scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
     else scan_bwd_body<T, W, Z, false>(a, bc0, p, smem);
 }
 
-// dB, dC [B][G][N][L]: the channel blocks' shares in a fixed order, turned back to token-contiguous.  A thread has one
-// token and one state.
+// What the backward kernel's blocks left in shares, each sum in a fixed order: the first `bcs` blocks take dB and dC
+// [B][G][N][L] from the channel blocks' shares (a thread has one token and a state of four, so writes are whole lines), the
+// others dA [D][N], dD and dbias [D] from those of all samples and chunks (rows 0 .. N-1 are dA's states, N is dD, N + 1
+// dbias; lanes run along the channels).
 template <typename T>
 __global__ void __launch_bounds__(256)
-scan_reduce_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC, int cb, int64_t stride, int N, int W,
-                      int64_t L, int64_t groups) {
-    const int64_t t = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int64_t bg = blockIdx.y;
-    if (t >= L) return;
-    for (int n = threadIdx.x >> 6; n < N; n += 4) {
-        const float* p = part + ((bg * groups + (t >> 3)) * W + (n >> 2)) * 64 + ((n >> 1) & 1) * 16 + (n & 1) * 8 + (t & 7);
-        float b = 0.f, c = 0.f;
-        for (int k = 0; k < cb; ++k) {
-            b += p[k * stride];
-            c += p[k * stride + 32];
+scan_reduce_kernel(const Scan a, int W, int bcs, float* __restrict__ dA, float* __restrict__ dD, float* __restrict__ dbias) {
+    if (blockIdx.x < (unsigned)bcs) {
+        const int across = (int)((a.L + 63) / 64);
+        const int64_t t = (int64_t)(blockIdx.x % across) * 64 + (threadIdx.x & 63);
+        const int64_t bg = blockIdx.x / across, groups = (int64_t)a.tiles * 2, stride = (int64_t)a.B * a.G * groups * W * 64;
+        if (t >= a.L) return;
+        T *dB = static_cast<T*>(a.dB), *dC = static_cast<T*>(a.dC);
+        for (int n = threadIdx.x >> 6; n < a.N; n += 4) {
+            const float* p = a.bcpart + ((bg * groups + (t >> 3)) * W + (n >> 2)) * 64 + ((n >> 1) & 1) * 16 + (n & 1) * 8 + (t & 7);
+            float b = 0.f, c = 0.f;
+            for (int k = 0; k < a.cb; ++k) {
+                b += p[k * stride];
+                c += p[k * stride + 32];
+            }
+            dB[(bg * a.N + n) * a.L + t] = Store<T>::put(b);
+            dC[(bg * a.N + n) * a.L + t] = Store<T>::put(c);
         }
-        dB[(bg * N + n) * L + t] = Store<T>::put(b);
-        dC[(bg * N + n) * L + t] = Store<T>::put(c);
+        return;
     }
-}
-
-// dA [D][N], dD [D], dbias [D]: the shares of all samples and chunks in a fixed order.  Rows 0 .. N-1 are dA's states,
-// N is dD, N + 1 dbias; lanes run along the channels.
-__global__ void __launch_bounds__(256)
-scan_reduce_params_kernel(const float* __restrict__ dApart, const float* __restrict__ dDpart, float* __restrict__ dA,
-                          float* __restrict__ dD, float* __restrict__ dbias, int n, int D, int N, int W) {
     __shared__ float red[16][17];
-    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
-    const int d = blockIdx.x * 16 + col, row = blockIdx.y;
+    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4, wide = (a.D + 15) / 16;
+    const int i = blockIdx.x - bcs, d = i % wide * 16 + col, row = i / wide, n = a.B * a.nchunk;
     float s = 0.f;
-    if (d < D)
-        for (int64_t c = slice; c < n; c += 16)
-            s += row < N ? dApart[(c * 4 * W + row) * D + d] : dDpart[(c * 2 + row - N) * D + d];
+    if (d < a.D) {
+        const float* p = row < a.N ? a.dApart + (int64_t)row * a.D + d : a.dDpart + (int64_t)(row - a.N) * a.D + d;
+        const int64_t step = (int64_t)(row < a.N ? 4 * W : 2) * a.D;
+#pragma unroll 8
+        for (int c = slice; c < n; c += 16) s += p[c * step];
+    }
     red[slice][col] = s;
     __syncthreads();
     for (int h = 8; h > 0; h >>= 1) {
         if (slice < h) red[slice][col] += red[slice + h][col];
         __syncthreads();
     }
-    if (slice != 0 || d >= D) return;
-    if (row < N) dA[(int64_t)d * N + row] = red[0][col];
-    else if (row == N) { if (dD) dD[d] = red[0][col]; }
+    if (slice != 0 || d >= a.D) return;
+    if (row < a.N) dA[(int64_t)d * a.N + row] = red[0][col];
+    else if (row == a.N) { if (dD) dD[d] = red[0][col]; }
     else if (dbias) dbias[d] = red[0][col];
 }
 
@@ -825,22 +840,31 @@ scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const f
 static bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
 static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 
-// How many chunks a row is cut into.  The chip holds 1024 blocks of the forward kernel (four to a compute unit) or 512 of
-// the backward kernel (two); more run in rounds, so 528 blocks take as long as 1024.  Chunks cost the pass over the
-// chunks' own states, 0.6 of the forward kernel's time and 0.2 of the backward's, and a block costs about half a tile beside
-// its tiles.  The number with the least rounds x tiles is taken, chunks of at least four tiles.
+// How many chunks a row is cut into.  A compute unit holds six blocks of the forward kernel or two of the backward.  k of them
+// side by side do not take k times one block's share of the vector pipe: a SIMD issues 39, 73, 84 and 93 multiply-adds a
+// clock and compute unit with one, two, four and eight waves, so one alone takes 2.4 shares (backward 1.9) and k take about
+// k + 1/2 (backward k).  Chunks cost the pass over their own states, 0.6 of the forward kernel's time and 0.2 of the
+// backward's, a block about half a tile beside its tiles, and the chain about three.  The number that costs least is
+// taken, chunks of at least two tiles.  Measured, 8 x 384 x 16384 bf16: forward 612, 529, 500, 468, 480 us with 10, 16, 21, 32, 48
+// chunks, backward 1804, 1227, 1125, 1095 with 5, 10, 21, 32; one 16384-token prompt of 192 channels 60 us with 512, 52 with 256.
 static void scan_plan(Scan* a, bool bwd) {
     a->Dg = a->D / a->G;
     a->cb = (int)cdiv(a->Dg, SC);
     a->tiles = (int)cdiv(a->L, ST);
-    const int64_t blocks = (int64_t)a->B * a->G * a->cb, slots = bwd ? 512 : 1536;
+    const int64_t blocks = (int64_t)a->B * a->G * a->cb;
+    const int held = bwd ? 2 : 6;
     const double again = bwd ? 1.2 : 1.6;
-    double best = (double)cdiv(blocks, slots) * (a->tiles + 0.5);
+    auto shares = [&](int64_t k) { return k == 0 ? 0.0 : bwd ? (k == 1 ? 1.9 : 2.0) : (k == 1 ? 2.4 : (double)k + 0.5); };
+    auto cost = [&](int64_t chunks, int64_t per) {
+        const int64_t k = cdiv(blocks * chunks, 256);
+        return ((double)(k / held) * shares(held) + shares(k % held)) * ((double)per + 0.5);
+    };
+    double best = cost(1, a->tiles);
     a->per_chunk = a->tiles;
-    for (int64_t n = 2; n <= a->tiles / 4 && n <= 1024 && blocks * n <= 4 * slots; ++n) {
-        const int64_t per = cdiv(a->tiles, n), real = cdiv(a->tiles, per);
-        const double cost = (double)cdiv(blocks * real, slots) * (per + 0.5) * again + 3.0;
-        if (cost < best) { best = cost; a->per_chunk = (int)per; }
+    for (int64_t n = 2; n <= a->tiles / 2 && n <= 1024 && blocks * n <= 4096; ++n) {
+        const int64_t per = cdiv(a->tiles, n);
+        const double c = cost(cdiv(a->tiles, per), per) * again + 3.0;
+        if (c < best) { best = c; a->per_chunk = (int)per; }
     }
     a->nchunk = (int)cdiv(a->tiles, a->per_chunk);
 }
@@ -861,7 +885,9 @@ static void scan_shape(Scan* a, const rst_scan_desc* s, bool bwd) {
     scan_plan(a, bwd);
 }
 
-// Scratch of a call, carved from the caller's workspace (base == null: only measured)
+// Scratch of a call, carved from the caller's workspace (base == null: only measured).  B and C laid out for the waves are
+// kept with the states for the backward pass, where there is one.
+static int64_t scan_bc_floats(const Scan& a) { return (int64_t)a.B * a.G * a.tiles * ST * scan_waves(a.N) * 8; }
 static size_t scan_carve(Scan* a, char* base, bool bwd) {
     const int W = scan_waves(a->N);
     size_t off = 0;
@@ -870,18 +896,22 @@ static size_t scan_carve(Scan* a, char* base, bool bwd) {
         off = (off + (size_t)floats * sizeof(float) + 255) & ~size_t(255);
         return p;
     };
-    const int64_t bcf = (int64_t)a->B * a->G * a->tiles * ST * W * 8, chunks = (int64_t)a->B * a->nchunk;
-    a->bc = take(bcf);
+    const int64_t chunks = (int64_t)a->B * a->nchunk;
+    if (!bwd) a->bc = take(scan_bc_floats(*a));
     if (a->nchunk > 1) {
         a->cst = take(chunks * 4 * W * a->D);
         a->cdt = take(chunks * a->D);
     }
     if (bwd) {
-        a->bcpart = take(bcf * a->cb);
+        a->bcpart = take(scan_bc_floats(*a) * a->cb);
         a->dApart = take(chunks * 4 * W * a->D);
         a->dDpart = take(chunks * 2 * a->D);
     }
     return off;
+}
+static void scan_saved(Scan* a, float* saved) {
+    a->bc = saved;
+    a->ckpt = saved + scan_bc_floats(*a);
 }
 
 template <typename T>
@@ -915,7 +945,6 @@ template <typename T, int W, bool Z>
 static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStream_t st) {
     const double n = (double)a.B * a.D * a.L;
     ProfScope prof(st, "scan_bwd", n * (16.0 * a.N + 28), sizeof(T) * n * (a.z ? 7 : 5));
-    RST_TRY(scan_prep<T>(a, W, st));
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
@@ -929,11 +958,9 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
     RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W, Z>), 64 * W, lds, &ks));
     hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a, a.bc);
     RST_LAUNCH_CHECK();
-    hipLaunchKernelGGL((scan_reduce_bc_kernel<T>), dim3((unsigned)cdiv(a.L, 64), a.B * a.G), dim3(256), 0, st, a.bcpart,
-                       static_cast<T*>(a.dB), static_cast<T*>(a.dC), a.cb, (int64_t)a.B * a.G * a.tiles * 2 * W * 64, a.N, W, a.L, (int64_t)a.tiles * 2);
-    RST_LAUNCH_CHECK();
-    hipLaunchKernelGGL(scan_reduce_params_kernel, dim3((unsigned)cdiv(a.D, 16), a.N + 2), dim3(256), 0, st, a.dApart, a.dDpart, dA, dD,
-                       dbias, a.B * a.nchunk, a.D, a.N, W);
+    const int64_t bcs = cdiv(a.L, 64) * a.B * a.G, all = bcs + cdiv(a.D, 16) * (a.N + 2);
+    RST_REQUIRE(all < (1ll << 31), "scan: grid out of range");
+    hipLaunchKernelGGL((scan_reduce_kernel<T>), dim3((unsigned)all), dim3(256), 0, st, a, W, (int)bcs, dA, dD, dbias);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
@@ -968,7 +995,7 @@ size_t rst_scan_saved_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_saved_bytes", s) != RST_OK) return 0;
     Scan a{};
     scan_shape(&a, s, true);
-    return (size_t)a.B * a.tiles * 4 * scan_waves(a.N) * a.D * sizeof(float);
+    return ((size_t)scan_bc_floats(a) + (size_t)a.B * a.tiles * 4 * scan_waves(a.N) * a.D) * sizeof(float);
 }
 size_t rst_scan_bwd_workspace_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_bwd_workspace_bytes", s) != RST_OK) return 0;
@@ -986,10 +1013,11 @@ int rst_scan_fwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     const size_t need = scan_carve(&a, nullptr, false);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_fwd: workspace too small (%zu < %zu)", workspace_bytes, need);
-    RST_REQUIRE(aligned256(workspace), "scan_fwd: workspace not aligned to 256 bytes");
+    RST_REQUIRE(aligned256(workspace) && aligned256(saved), "scan_fwd: workspace or saved not aligned to 256 bytes");
     scan_carve(&a, static_cast<char*>(workspace), false);
     a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
-    a.h0 = state_in; a.y = y; a.last = state_out; a.ckpt = saved;
+    a.h0 = state_in; a.y = y; a.last = state_out;
+    if (saved) scan_saved(&a, saved);
     const int W = scan_waves(a.N);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define FWD(T, W_) (a.z ? scan_fwd_t<T, W_, true>(a, st) : scan_fwd_t<T, W_, false>(a, st))
@@ -1007,10 +1035,11 @@ int rst_scan_bwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     const size_t need = scan_carve(&a, nullptr, true);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_bwd: workspace too small (%zu < %zu)", workspace_bytes, need);
-    RST_REQUIRE(aligned256(workspace), "scan_bwd: workspace not aligned to 256 bytes");
+    RST_REQUIRE(aligned256(workspace) && aligned256(saved), "scan_bwd: workspace or saved not aligned to 256 bytes");
     scan_carve(&a, static_cast<char*>(workspace), true);
     a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
-    a.ckpt = const_cast<float*>(saved); a.dy = dy; a.dlast = dstate_out;
+    scan_saved(&a, const_cast<float*>(saved));
+    a.dy = dy; a.dlast = dstate_out;
     a.dx = out->x; a.ddelta = out->delta; a.dB = out->B; a.dC = out->C; a.dz = out->z; a.dh0 = dstate_in;
     const int W = scan_waves(a.N);
     hipStream_t st = static_cast<hipStream_t>(stream);

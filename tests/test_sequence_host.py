@@ -190,7 +190,7 @@ def test_c_entry_points_refuse():
 
     def desc(B=1, D=4, G=1, N=8, L=10, dtype=0):
         return ctypes.byref(_lib.ScanDesc(B, D, G, N, L, dtype, 1))
-    for kw in (dict(B=0), dict(D=0), dict(L=0), dict(N=0), dict(N=33), dict(G=3), dict(G=0), dict(dtype=7), dict(B=70000), dict(L=1 << 32)):
+    for kw in (dict(B=0), dict(D=0), dict(L=0), dict(N=0), dict(N=33), dict(G=3), dict(G=0), dict(dtype=7), dict(B=70000), dict(L=(1 << 24) + 1)):
         assert lib.rst_scan_workspace_bytes(desc(**kw)) == 0, kw
         assert lib.rst_scan_saved_bytes(desc(**kw)) == 0 and lib.rst_scan_bwd_workspace_bytes(desc(**kw)) == 0
     ins = _lib.ScanInputs(p, p, p, p, p, None, None, None)
