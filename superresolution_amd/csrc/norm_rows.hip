@@ -257,10 +257,17 @@ size_t norm_rows_bwd_ws_bytes(int64_t rows, int C) {
     return (size_t)NR_BWD_BLOCKS * 2 * (size_t)C * sizeof(float);
 }
 
+// The pairs that the plan comes to for some length, fp32 (4 values a vector) or bf16 (8)
+static constexpr bool nr_reached(int vec, int lpr, int nv) {
+    if (lpr == 256) return 256 * nv * vec <= NR_MAX_C;
+    if (lpr == 8) return nv <= (vec == 8 ? 3 : 4);
+    return vec == 8 ? nv == 2 || nv == 3 : nv == 3 || nv == 4;
+}
 #define NR_CASES(X, ...)                                                                                                 \
-    X(8, 1, __VA_ARGS__) X(8, 2, __VA_ARGS__) X(8, 3, __VA_ARGS__) X(8, 4, __VA_ARGS__) X(16, 3, __VA_ARGS__)              \
-    X(16, 4, __VA_ARGS__) X(32, 3, __VA_ARGS__) X(32, 4, __VA_ARGS__) X(64, 3, __VA_ARGS__) X(64, 4, __VA_ARGS__)          \
-    X(256, 2, __VA_ARGS__) X(256, 4, __VA_ARGS__) X(256, 8, __VA_ARGS__)
+    X(8, 1, __VA_ARGS__) X(8, 2, __VA_ARGS__) X(8, 3, __VA_ARGS__) X(8, 4, __VA_ARGS__) X(16, 2, __VA_ARGS__)              \
+    X(16, 3, __VA_ARGS__) X(16, 4, __VA_ARGS__) X(32, 2, __VA_ARGS__) X(32, 3, __VA_ARGS__) X(32, 4, __VA_ARGS__)          \
+    X(64, 2, __VA_ARGS__) X(64, 3, __VA_ARGS__) X(64, 4, __VA_ARGS__) X(256, 2, __VA_ARGS__) X(256, 4, __VA_ARGS__)        \
+    X(256, 8, __VA_ARGS__)
 
 // The kernel for a plan: every length of a row has exactly one.
 #define NR_DISPATCH(KERNEL, LDS, GRID, ...)                                                                               \
@@ -275,7 +282,7 @@ size_t norm_rows_bwd_ws_bytes(int64_t rows, int C) {
     } while (0)
 #define NR_CASE_OF(L_, N_, KERNEL, LDS, GRID, ...)                                                                        \
     case L_ * 16 + N_:                                                                                                   \
-        if constexpr (L_ == 256 ? L_ * N_ * V <= NR_MAX_C : N_ * V <= 24)                                                                         \
+        if constexpr (nr_reached(V, L_, N_))                                                                         \
             hipLaunchKernelGGL((KERNEL<T, V, L_, N_>), dim3((unsigned)(GRID)), dim3(256), LDS, st, __VA_ARGS__);          \
         break;
 

@@ -861,7 +861,10 @@ static void scan_plan(Scan* a, bool bwd) {
     };
     double best = cost(1, a->tiles);
     a->per_chunk = a->tiles;
-    for (int64_t n = 2; n <= a->tiles / 2 && n <= 1024 && blocks * n <= 4096; ++n) {
+    for (int64_t k = 1; k <= 16; ++k) {                                    // k blocks a compute unit
+        int64_t n = 256 * k / blocks;
+        if (n > a->tiles / 2) n = a->tiles / 2;
+        if (n < 2) continue;
         const int64_t per = cdiv(a->tiles, n);
         const double c = cost(cdiv(a->tiles, per), per) * again + 3.0;
         if (c < best) { best = c; a->per_chunk = (int)per; }

@@ -26,37 +26,38 @@ from ._lib import ScanDesc, ScanGrads, ScanInputs, check
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MAX_STATES = 32          # of a channel of the scan
 MAX_NORM_WIDTH = 8192
+MAX_TOKENS = 1 << 24     # of a row of the scan
 
 
 # ----------------------------------------------------------------------------
 # plumbing
 # ----------------------------------------------------------------------------
-def _act(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+def _act(t: torch.Tensor, op: str, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
     """An activation: fp32 or bf16 on a ROCm device, of `like`'s type and device."""
     if not t.is_cuda:
-        raise RuntimeError(f"{name}: tensor is on {t.device}; this operator only runs on a ROCm GPU "
+        raise RuntimeError(f"{op} {what}: tensor is on {t.device}; this operator only runs on a ROCm GPU "
                            "(there is no CPU fallback)")
     if t.dtype not in _DTYPES:
-        raise RuntimeError(f"{name}: dtype {t.dtype} not supported (fp32 or bf16)")
+        raise RuntimeError(f"{op} {what}: dtype {t.dtype} not supported (fp32 or bf16)")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise RuntimeError(f"{name}: {t.dtype} on {t.device}, but x is {like.dtype} on {like.device}")
+        raise RuntimeError(f"{op} {what}: {t.dtype} on {t.device}, but x is {like.dtype} on {like.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _par(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> Optional[torch.Tensor]:
+def _par(t: Optional[torch.Tensor], op: str, what: str, like: torch.Tensor) -> Optional[torch.Tensor]:
     """A parameter or a state of the scan: fp32 on `like`'s device, or None."""
     if t is None:
         return None
     if t.device != like.device:
-        raise RuntimeError(f"{name}: tensor is on {t.device}, but x is on {like.device}")
+        raise RuntimeError(f"{op} {what}: tensor is on {t.device}, but x is on {like.device}")
     if t.dtype != torch.float32:
-        raise RuntimeError(f"{name}: dtype {t.dtype} not supported (fp32 only)")
+        raise RuntimeError(f"{op} {what}: dtype {t.dtype} not supported (fp32 only)")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _shape(t: Optional[torch.Tensor], name: str, want: tuple) -> None:
-    if t is not None and tuple(t.shape) != want:
-        raise RuntimeError(f"{name}: shape {tuple(t.shape)}, expected {want}")
+def _shape(t: Optional[torch.Tensor], op: str, what: str, want: tuple) -> None:
+    if t is not None and t.shape != want:
+        raise RuntimeError(f"{op} {what}: shape {tuple(t.shape)}, expected {want}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -137,7 +138,7 @@ class _LayerNormFn(torch.autograd.Function):
         x, weight = ctx.saved_tensors
         if x.numel() == 0:
             return torch.zeros_like(x), torch.zeros_like(weight), torch.zeros_like(weight) if ctx.with_bias else None, None
-        dy = _act(dy, "layernorm dy", x)
+        dy = _act(dy, "layernorm", "dy", x)
         dx, dw = torch.empty_like(x), torch.empty_like(weight)
         db = torch.empty_like(weight) if ctx.with_bias else None
         rows, C = x.numel() // x.shape[-1], x.shape[-1]
@@ -157,10 +158,10 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
         raise RuntimeError(f"layernorm: x {tuple(x.shape)} (the last dimension: 1 to {MAX_NORM_WIDTH})")
     if not eps >= 0:
         raise RuntimeError(f"layernorm: eps={eps} is negative or no number")
-    x = _act(x, "layernorm x")
-    _shape(weight, "layernorm weight", (x.shape[-1],))
-    _shape(bias, "layernorm bias", (x.shape[-1],))
-    weight, bias = _par(weight, "layernorm weight", x), _par(bias, "layernorm bias", x)
+    x = _act(x, "layernorm", "x")
+    _shape(weight, "layernorm", "weight", (x.shape[-1],))
+    _shape(bias, "layernorm", "bias", (x.shape[-1],))
+    weight, bias = _par(weight, "layernorm", "weight", x), _par(bias, "layernorm", "bias", x)
     if _wants_grad(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps))
@@ -197,14 +198,14 @@ class _CausalConvFn(torch.autograd.Function):
         x, weight, bias, state = ctx.saved_tensors
         B, D, L = x.shape
         W = weight.shape[1]
-        dend = None if dend is None else _act(dend, "causal_conv1d final state's gradient", x)
+        dend = None if dend is None else _act(dend, "causal_conv1d", "final state's gradient", x)
         dstate = None if state is None else torch.empty_like(state)
         if x.numel() == 0:
             if dstate is not None:
                 dstate.zero_() if dend is None else dstate.copy_(dend)
             return (torch.zeros_like(x), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), dstate, None,
                     None)
-        dy = torch.zeros_like(x) if dy is None else _act(dy, "causal_conv1d dy", x)
+        dy = torch.zeros_like(x) if dy is None else _act(dy, "causal_conv1d", "dy", x)
         dx, dw = torch.empty_like(x), torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         nb = _lib.load().rst_causal_conv1d_bwd_workspace_bytes(B, D, L)
@@ -217,14 +218,14 @@ class _CausalConvFn(torch.autograd.Function):
 def _conv_args(name, x, weight, bias, activation):
     if activation not in (None, "silu"):
         raise RuntimeError(f"{name}: activation {activation!r} (None or 'silu')")
-    x = _act(x, f"{name} x")
+    x = _act(x, name, "x")
     if weight.dim() == 3 and weight.shape[1] == 1:          # a depthwise nn.Conv1d's
         weight = weight.squeeze(1)
     D = x.shape[1]
     if weight.dim() != 2 or weight.shape[0] != D or not 2 <= weight.shape[1] <= 4:
         raise RuntimeError(f"{name}: weight {tuple(weight.shape)} does not fit {D} channels and 2 to 4 taps")
-    _shape(bias, f"{name} bias", (D,))
-    return x, _par(weight, f"{name} weight", x), _par(bias, f"{name} bias", x)
+    _shape(bias, name, "bias", (D,))
+    return x, _par(weight, name, "weight", x), _par(bias, name, "bias", x)
 
 
 def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -238,8 +239,8 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise RuntimeError(f"causal_conv1d: x {tuple(x.shape)} (batch, channel, token)")
     x, weight, bias = _conv_args("causal_conv1d", x, weight, bias, activation)
     if initial_state is not None:
-        _shape(initial_state, "causal_conv1d initial_state", (x.shape[0], x.shape[1], weight.shape[1] - 1))
-        initial_state = _act(initial_state, "causal_conv1d initial_state", x)
+        _shape(initial_state, "causal_conv1d", "initial_state", (x.shape[0], x.shape[1], weight.shape[1] - 1))
+        initial_state = _act(initial_state, "causal_conv1d", "initial_state", x)
     if _wants_grad(x, weight, bias, initial_state):
         return _CausalConvFn.apply(x, weight, bias, initial_state, activation == "silu", bool(return_final_state))
     y, end = _conv_forward(x, weight, bias, initial_state, activation == "silu", return_final_state)
@@ -256,8 +257,8 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
         raise RuntimeError("causal_conv1d_update is inference only: call it under torch.no_grad()")
     x, weight, bias = _conv_args("causal_conv1d_update", x, weight, bias, activation)
     B, D, W = x.shape[0], x.shape[1], weight.shape[1]
-    _shape(state, "causal_conv1d_update state", (B, D, W - 1))
-    state, out = _act(state, "causal_conv1d_update state", x), _next_state(state, state_out, "causal_conv1d_update")
+    _shape(state, "causal_conv1d_update", "state", (B, D, W - 1))
+    state, out = _act(state, "causal_conv1d_update", "state", x), _next_state(state, state_out, "causal_conv1d_update")
     y = torch.empty_like(x)
     if x.numel():
         _call("rst_causal_conv1d_update", x, x.data_ptr(), _DTYPES[x.dtype], state.data_ptr(), out.data_ptr(), weight.data_ptr(),
@@ -309,13 +310,13 @@ class _ScanFn(torch.autograd.Function):
         _first_order_only("selective_scan")
         *ins, saved = ctx.saved_tensors
         x, delta, A, B, C, D, z, delta_bias = ins
-        dlast = _par(dlast, "selective_scan last state's gradient", x)
+        dlast = _par(dlast, "selective_scan", "last state's gradient", x)
         dh0 = torch.empty((x.shape[0], x.shape[1], A.shape[1]), dtype=torch.float32, device=x.device) if ctx.has_h0 else None
         if x.numel() == 0:
             if dh0 is not None:
                 dh0.zero_() if dlast is None else dh0.copy_(dlast)
             return tuple(None if t is None else torch.zeros_like(t) for t in ins) + (dh0, None, None)
-        dy = torch.zeros_like(x) if dy is None else _act(dy, "selective_scan dy", x)
+        dy = torch.zeros_like(x) if dy is None else _act(dy, "selective_scan", "dy", x)
         grads = [None if t is None else torch.empty_like(t) for t in ins]
         desc, inputs, outs = _scan_desc(x, A, B, ctx.softplus), _scan_inputs(*ins), ScanGrads(*[_ptr(g) for g in grads])
         ref = ctypes.byref(desc)
@@ -327,7 +328,7 @@ class _ScanFn(torch.autograd.Function):
 
 
 def _scan_args(name, x, delta, A, B, C, D, z, delta_bias):
-    x = _act(x, f"{name} x")
+    x = _act(x, name, "x")
     batch, chan, tail = x.shape[0], x.shape[1], tuple(x.shape[2:])
     if A.dim() != 2 or A.shape[0] != chan or not 1 <= A.shape[1] <= MAX_STATES:
         raise RuntimeError(f"{name}: A {tuple(A.shape)} does not fit {chan} channels and 1 to {MAX_STATES} states")
@@ -338,14 +339,14 @@ def _scan_args(name, x, delta, A, B, C, D, z, delta_bias):
     groups = B.shape[1] if B.dim() == x.dim() + 1 else 0
     if groups < 1 or chan % groups:
         raise RuntimeError(f"{name}: B {tuple(B.shape)}: {chan} channels are not divisible into its groups")
-    _shape(B, f"{name} B", (batch, groups, A.shape[1]) + tail)
-    _shape(C, f"{name} C", (batch, groups, A.shape[1]) + tail)
-    _shape(delta, f"{name} delta", tuple(x.shape))
-    _shape(z, f"{name} z", tuple(x.shape))
-    _shape(D, f"{name} D", (chan,))
-    _shape(delta_bias, f"{name} delta_bias", (chan,))
-    return (x, _act(delta, f"{name} delta", x), _par(A, f"{name} A", x), _act(B, f"{name} B", x), _act(C, f"{name} C", x),
-            _par(D, f"{name} D", x), None if z is None else _act(z, f"{name} z", x), _par(delta_bias, f"{name} delta_bias", x))
+    _shape(B, name, "B", (batch, groups, A.shape[1]) + tail)
+    _shape(C, name, "C", (batch, groups, A.shape[1]) + tail)
+    _shape(delta, name, "delta", x.shape)
+    _shape(z, name, "z", x.shape)
+    _shape(D, name, "D", (chan,))
+    _shape(delta_bias, name, "delta_bias", (chan,))
+    return (x, _act(delta, name, "delta", x), _par(A, name, "A", x), _act(B, name, "B", x), _act(C, name, "C", x),
+            _par(D, name, "D", x), None if z is None else _act(z, name, "z", x), _par(delta_bias, name, "delta_bias", x))
 
 
 def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
@@ -361,16 +362,18 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     `x`, `delta`, `z`: (batch, channel, token).  `A`: (channel, state), up to 32 states.  `B`, `C`: (batch, group, state,
     token), channel d reads group ``d // (channels / groups)`` -- or (batch, state, token) for one group.  `D`,
     `delta_bias`: (channel).  `initial_state` and, with `return_last_state`, the second result: (batch, channel, state),
-    fp32.  A token leaves the state alone where its step size is zero (`delta` = -inf under the softplus, and a finite
+    fp32.  At most 2^24 tokens a call.  A token leaves the state alone where its step size is zero (`delta` = -inf under the softplus, and a finite
     `x`): that is how sequences of different lengths are padded.  Differentiable in every tensor; for that the states
     of every 16th token are kept.  Counterpart in the reference: the scan that model/basicsr/archs/mambairv2_arch.py:384-390
     calls, with the same order of its first six arguments."""
     if x.dim() != 3:
         raise RuntimeError(f"selective_scan: x {tuple(x.shape)} (batch, channel, token)")
+    if x.shape[2] > MAX_TOKENS:
+        raise RuntimeError(f"selective_scan: {x.shape[2]} tokens (at most {MAX_TOKENS}: carry the state on in pieces)")
     args = _scan_args("selective_scan", x, delta, A, B, C, D, z, delta_bias)
     x, A = args[0], args[2]
-    _shape(initial_state, "selective_scan initial_state", (x.shape[0], x.shape[1], A.shape[1]))
-    h0 = _par(initial_state, "selective_scan initial_state", x)
+    _shape(initial_state, "selective_scan", "initial_state", (x.shape[0], x.shape[1], A.shape[1]))
+    h0 = _par(initial_state, "selective_scan", "initial_state", x)
     if _wants_grad(*args, h0):
         return _ScanFn.apply(*args, h0, bool(delta_softplus), bool(return_last_state))
     y, last, _ = _scan_forward(*args, h0, delta_softplus, return_last_state, False)
@@ -388,8 +391,8 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     if _wants_grad(state, x, delta, A, B, C, D, z, delta_bias):
         raise RuntimeError("selective_scan_update is inference only: call it under torch.no_grad()")
     x, delta, A, B, C, D, z, delta_bias = _scan_args("selective_scan_update", x, delta, A, B, C, D, z, delta_bias)
-    _shape(state, "selective_scan_update state", (x.shape[0], x.shape[1], A.shape[1]))
-    state, out = _par(state, "selective_scan_update state", x), _next_state(state, state_out, "selective_scan_update")
+    _shape(state, "selective_scan_update", "state", (x.shape[0], x.shape[1], A.shape[1]))
+    state, out = _par(state, "selective_scan_update", "state", x), _next_state(state, state_out, "selective_scan_update")
     y = torch.empty_like(x)
     if x.numel():
         desc, ins = _scan_desc(x, A, B, delta_softplus), _scan_inputs(x, delta, A, B, C, D, z, delta_bias)

@@ -39,7 +39,9 @@ def _leaf(t):
 
 # ---- norm ------------------------------------------------------------------------------------------------------
 NORM_SHAPES = [(1, 1), (3, 2), (2, 3), (5, 4), (4, 7), (5, 8), (7, 9), (1, 16), (33, 24), (4, 33), (70, 48), (65, 96), (3, 181), (9, 192),
-               (2, 384), (9, 513), (3, 1025), (2, 2049), (3, 4099), (2, 8191), (2, 8192), (1500, 64)]
+               (2, 384), (9, 513), (3, 1025), (2, 2049), (3, 4099), (2, 8191), (2, 8192), (1500, 64),
+               # one at least for every number of lanes and vectors a row is dealt to, in either type
+               (40, 17), (40, 25), (40, 130), (20, 200), (20, 250), (20, 300), (20, 400), (20, 500), (9, 700), (9, 1000), (9, 1500), (9, 1600), (9, 2000), (5, 3000), (5, 5000)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -490,3 +492,101 @@ def test_inputs_are_left_alone():
     (y.float().sum() + last.sum()).backward()
     for k, v in leaves.items():
         assert torch.equal(v.detach(), kept[k]), k
+
+
+def test_two_streams_at_once():
+    """Calls of two streams overlap: scratch is a call's own."""
+    g = _gen(26)
+    cs = [{k: (None if v is None else v.cuda()) for k, v in _scan_case(g, 2, 96, 1, 16, 2000, F32, True, True, True).items()} for _ in range(2)]
+    dy = torch.randn(2, 96, 2000, device="cuda")
+    cw = torch.randn(96, 4, device="cuda")
+
+    def work(c):
+        leaves = [c[k].detach().requires_grad_(True) for k in ("x", "A", "B")]
+        u = sequence.causal_conv1d(leaves[0], cw.detach().requires_grad_(True), activation="silu")
+        y = sequence.selective_scan(u, c["delta"], leaves[1], leaves[2], c["C"], c["D"], z=c["z"], delta_bias=c["delta_bias"],
+                                    delta_softplus=True, initial_state=c["h0"])
+        y = sequence.layernorm(y, dy[0, 0].detach().requires_grad_(True))
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    want = [work(c) for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for c, st in zip(cs, streams):
+            with torch.cuda.stream(st):
+                got.append(work(c))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_gradients_are_first_order_only():
+    x, w = torch.randn(3, 8, device="cuda", requires_grad=True), torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="first-order"):
+        torch.autograd.grad(sequence.layernorm(x, w).sum(), x, create_graph=True)
+    x = torch.randn(1, 4, 9, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="first-order"):
+        torch.autograd.grad(sequence.causal_conv1d(x, torch.ones(4, 3, device="cuda")).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="first-order"):
+        torch.autograd.grad(sequence.selective_scan(x, x.detach().abs(), -torch.ones(4, 2, device="cuda"), torch.ones(1, 2, 9, device="cuda"),
+                                                    torch.ones(1, 2, 9, device="cuda")).sum(), x, create_graph=True)
+
+
+def test_unused_outputs():
+    """A backward pass that only the last state, or only the result, feeds."""
+    g = _gen(27)
+    c = {k: _leaf(v) for k, v in _scan_case(g, 1, 5, 1, 3, 12, F32, False, True, True).items()}
+    run = lambda: sequence.selective_scan(*_scan_args(c), delta_bias=c["delta_bias"], delta_softplus=True, initial_state=c["h0"],
+                                          return_last_state=True)
+    y, last = run()
+    gx, gz = torch.autograd.grad(last.sum(), [c["x"], c["C"]])
+    cpu = {k: (None if v is None else v.detach().cpu()) for k, v in c.items()}
+    want, mag = so.scan(*_scan_args(cpu), None, cpu["delta_bias"], True, cpu["h0"], torch.zeros(1, 5, 12), torch.ones(1, 5, 3))
+    so.within(gx, want["dx"], mag["dx"], 8 * 12 + 90, "dx")
+    assert torch.equal(gz, torch.zeros_like(gz))
+    y, last = run()
+    gx, = torch.autograd.grad(y.sum(), [c["x"]])
+    want, mag = so.scan(*_scan_args(cpu), None, cpu["delta_bias"], True, cpu["h0"], torch.ones(1, 5, 12))
+    so.within(gx, want["dx"], mag["dx"], 8 * 12 + 90, "dx")
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values a tensor: what stands at the end is what a call on the end alone gives."""
+    C, rows = 1000, 2_200_000
+    x = torch.zeros(rows, C, dtype=BF16, device="cuda")
+    x[-5:] = torch.randn(5, C, device="cuda").to(BF16)
+    w = torch.linspace(0.5, 1.5, C, device="cuda")
+    tail = x[-5:].clone().requires_grad_(True)
+    small = sequence.layernorm(tail, w)
+    small.backward(tail.detach())
+    x.requires_grad_(True)
+    y = sequence.layernorm(x, w)
+    assert torch.equal(y[-5:], small) and not y[:5].any()
+    y.backward(x.detach())
+    assert torch.equal(x.grad[-5:], tail.grad)
+    del x, y, small
+
+    L = 1 << 27
+    x = torch.zeros(3, 6, L, dtype=BF16, device="cuda")
+    x[-1, -1, -100:] = torch.randn(100, device="cuda").to(BF16)
+    cw, cb = torch.randn(6, 4, device="cuda"), torch.randn(6, device="cuda")
+    y, end = sequence.causal_conv1d(x, cw, cb, activation="silu", return_final_state=True)
+    small = sequence.causal_conv1d(x[-1:, -1:, -90:], cw[-1:], cb[-1:], initial_state=x[-1:, -1:, -93:-90].contiguous(), activation="silu")
+    assert torch.equal(y[-1, -1, -90:], small[0, 0]) and torch.equal(end[-1, -1], x[-1, -1, -3:])
+    del x, y, small
+
+    L = 1 << 22
+    B = 9
+    x = torch.zeros(B, 64, L, dtype=BF16, device="cuda")
+    x[-1, :, -200:] = torch.randn(64, 200, device="cuda").to(BF16)
+    delta = torch.full((1, 1, 1), 0.3, dtype=BF16, device="cuda").expand(B, 64, L).contiguous()
+    A = -torch.linspace(0.5, 2.0, 64 * 4, device="cuda").view(64, 4)
+    bc = torch.ones(1, 1, 1, 1, dtype=BF16, device="cuda").expand(B, 1, 4, L).contiguous()
+    y, last = sequence.selective_scan(x, delta, A, bc, bc, return_last_state=True)
+    # before the last 200 tokens nothing has entered the state: the same as those tokens alone.  The step size and the products
+    # are the same; the chunks of the two calls start elsewhere, which costs a few roundings of each of them
+    want, end = sequence.selective_scan(x[-1:, :, -200:], delta[:1, :, :200], A, bc[:1, ..., :200], bc[:1, ..., :200], return_last_state=True)
+    assert float((y[-1, :, -200:].float() - want[0].float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+    assert float((last[-1] - end[0]).abs().max()) <= 64 * 2.0 ** -24 * float(end.abs().max())
+    assert not y[-1, :, :-200].any() and not y[0].any()

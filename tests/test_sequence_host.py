@@ -205,3 +205,9 @@ def test_c_entry_points_refuse():
     assert lib.rst_scan_bwd(desc(), ctypes.byref(ins), None, p, None, ctypes.byref(outs), None, p, need, None) == 1 and "null" in err()
     assert lib.rst_scan_update(desc(), ctypes.byref(ins), p, p, p, None) == 1 and "one token" in err()
     assert ctypes.sizeof(_lib.ScanDesc) == 32 and ctypes.sizeof(_lib.ScanInputs) == 64
+
+
+def test_the_longest_row(fake):
+    with pytest.raises(RuntimeError, match="at most 16777216"):
+        sequence.selective_scan(fake(1, 2, (1 << 24) + 1), fake(1, 2, (1 << 24) + 1), fake(2, 1), fake(1, 1, 1, (1 << 24) + 1),
+                                fake(1, 1, 1, (1 << 24) + 1))
