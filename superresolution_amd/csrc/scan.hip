@@ -47,16 +47,13 @@ struct Scan {
     int softplus;
 };
 
-// log(1 + e^v).  e^v: the rounding of v log2 e is given back (it is up to |v| 2^-24 of the result).  w = 1 + e^v loses the
-// low bits of a small e^v; below 1 they are worth c = e^v - (w - 1) itself (c / w up to one more rounding), above nothing.
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v|.  w = 1 + e loses the low bits of a small e; c = e - (w - 1), an exact
+// difference, gives them back (c / w would be right, and is the same to one more rounding).  The rounding of |v| log2 e is
+// left in: it is worth at most |v| 2^-24 of e, 2 to 3e-7 of a step size of 0.001, and giving it back costs a third of the
+// function again.  -inf gives an exact zero.
 __device__ __forceinline__ float softplus(float v) {
-    const float t = v * LOG2E, low = fmaf(v, LOG2E, -t) * 0.6931471805599453f;
-    float e = __builtin_amdgcn_exp2f(t);
-    e = e > 0.f ? fmaf(e, low, e) : 0.f;                                   // (v = -inf: low is no number)
-    const float w = 1.0f + e;
-    const float c = e < 1.0f ? e - (w - 1.0f) : 0.f;
-    const float l = fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, c);
-    return v <= 20.f ? l : v;                                              // (and v itself where it is no number)
+    const float e = __builtin_amdgcn_exp2f(-fabsf(v) * LOG2E), w = 1.0f + e;
+    return fmaxf(v, 0.f) + fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, e - (w - 1.0f));
 }
 
 // which chunk, sample, group and channels a block has
@@ -191,15 +188,19 @@ __device__ __forceinline__ void load_rates(const Scan& a, int d, bool ok, int wa
     for (int s = 0; s < 4; ++s) A[s] = ok && wave * 4 + s < a.N ? a.A[(int64_t)d * a.N + wave * 4 + s] : 0.f;
 }
 
-// dt of four tokens: zero where there is no channel or token, so that nothing there moves a state
+// dt of four tokens: zero where there is no channel (all: the block has 64) or token, so that nothing there moves a state
 template <typename T>
 __device__ __forceinline__ void step_sizes(const Scan& a, const Quad<T>& qd, float bias, const ScanTile& tl, int q, bool ok,
-                                           float (&raw)[4], float (&dt)[4]) {
+                                           bool all, float (&raw)[4], float (&dt)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         raw[i] = qd.r.get(i) + bias;
         dt[i] = step_size(a, raw[i]);
-        if (!ok || q * 4 + i >= tl.left) dt[i] = 0.f;
+    }
+    if (!all || !tl.full()) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (!ok || q * 4 + i >= tl.left) dt[i] = 0.f;
     }
 }
 template <typename T>
@@ -217,7 +218,8 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     const ScanPlace p(a, a.nchunk - 1, REV ? 1 : 0);
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
     const bool ok = p.cb * SC + p.lane < a.Dg;
-    float A[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+    const bool whole = p.cb * SC + SC <= a.Dg;
+    float A[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sum[NI];                       // sum: of the dt of the thread's own tokens
     load_rates(a, d, ok, p.wave, A);
 #pragma unroll
     for (int s = 0; s < 4; ++s) A[s] *= LOG2E;
@@ -239,6 +241,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     for (int k = 0; k < NI; ++k) {
         it[k].set(a, p, k);
         bias[k] = a.dbias && it[k].ok ? a.dbias[it[k].d] : 0.f;
+        sum[k] = 0.f;
     }
     fetch(REV ? t1 - 1 : t0);
     for (int n = 0; n < t1 - t0; ++n) {
@@ -247,14 +250,15 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             float raw[4], dt[4];
-            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, raw, dt);
+            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, whole, raw, dt);
+            sum[k] += (dt[0] + dt[1]) + (dt[2] + dt[3]);
             if (ScanItem<W>::has(k)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float u = qx[k].r.get(i);
                     if constexpr (REV) {
                         if constexpr (Z) u *= gate_of(qz[k], i);
-                        u = it[k].ok ? u : 0.f;
+                        if (!whole && !it[k].ok) u = 0.f;
                     } else u *= dt[i];
                     dts[it[k].q * 4 + i][it[k].r] = dt[i];
                     us[it[k].q * 4 + i][it[k].r] = u;
@@ -283,7 +287,6 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = REV ? 3 - i : i;
-                sum += dt[j];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     const float decay = __builtin_amdgcn_exp2f(dt[j] * A[s]);
@@ -294,28 +297,33 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
         }
         __syncthreads();
     }
+    const int64_t c = (int64_t)p.b * a.nchunk + p.chunk;
     if (ok) {
-        const int64_t c = (int64_t)p.b * a.nchunk + p.chunk;
 #pragma unroll
         for (int s = 0; s < 4; ++s) a.cst[(c * 4 * W + p.wave * 4 + s) * a.D + d] = h[s];
-        if (p.wave == 0) a.cdt[c * a.D + d] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) sum[k] += __shfl_xor(sum[k], off, 64);
+        if (it[k].ok && it[k].q == 0) a.cdt[c * a.D + it[k].d] = sum[k];
     }
 }
 
 // ---- the chunks' own states, one behind the other: cst[c] becomes the state that chunk c starts from (REV: the
-// state's gradient behind it).  A block has 64 channels and one state; its 16 waves take 16 runs of chunks side by side,
-// chain the runs through LDS and walk their run again.  (Chained in front of every chunk by the scan's own blocks, the
+// state's gradient behind it).  A block has 64 channels and one state; its waves take a run of chunks each, side by side,
+// chain the runs through LDS and walk their run again: four waves for up to 32 chunks, which then stay in registers, else 16.  (Chained in front of every chunk by the scan's own blocks, the
 // states are read as often as there are chunks: 503 MB from the caches for 256 chunks of 192 channels, 45 us instead of 20.)
-template <bool REV>
-__global__ void __launch_bounds__(1024)
+template <bool REV, int RUNS>
+__global__ void __launch_bounds__(64 * RUNS)
 scan_chain_kernel(const Scan a, int states) {
-    __shared__ float sums[16][64], own[16][64];
+    __shared__ float sums[RUNS][64], own[RUNS][64];
     const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
     const int d = blockIdx.x * 64 + lane, n = blockIdx.y, b = blockIdx.z;
     const bool ok = d < a.D;
     const int dr = ok ? d : 0;
     const float A = n < a.N ? a.A[(int64_t)dr * a.N + n] * LOG2E : 0.f;
-    const int per = (a.nchunk + 15) / 16, c0 = run * per, c1 = c0 + per < a.nchunk ? c0 + per : a.nchunk;
+    const int per = (a.nchunk + RUNS - 1) / RUNS, c0 = run * per, c1 = c0 + per < a.nchunk ? c0 + per : a.nchunk;
     float* st = a.cst + ((int64_t)b * a.nchunk * states + n) * a.D;        // chunk c: + c states D
     const float* dt = a.cdt + (int64_t)b * a.nchunk * a.D;
     // chunk c on the way; the last one has nothing behind it and left no state
@@ -372,7 +380,7 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
     __shared__ float dts[ST][SROW], us[ST][SROW], part[W][ST][SROW];
     const ScanPlace p(a, a.nchunk, 0);
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
-    const bool ok = p.cb * SC + p.lane < a.Dg;
+    const bool ok = p.cb * SC + p.lane < a.Dg, whole = p.cb * SC + SC <= a.Dg;
     const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
     ScanItem<W> it[NI];
     float bias[NI], skip[NI];
@@ -407,7 +415,7 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             float raw[4], dt[4];
-            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, raw, dt);
+            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, whole, raw, dt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[k][i] = qx[k].r.get(i);
@@ -566,11 +574,11 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             float dt[4];
-            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, raw[k], dt);
+            step_sizes<T>(a, qd[k], bias[k], tl, it[k].q, it[k].ok, WHOLE, raw[k], dt);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[k][i] = qx[k].r.get(i);
-                float e = it[k].ok ? qy[k].r.get(i) : 0.f;
+                float e = WHOLE || it[k].ok ? qy[k].r.get(i) : 0.f;
                 if constexpr (Z) {
                     const float z = qz[k].r.get(i), q = sigmoid(z);
                     slope[k][i] = e * (q * fmaf(z, 1.0f - q, 1.0f));
@@ -697,7 +705,8 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                 Quad<T>::put(a.dz, tl, it[k].row, it[k].q, it[k].ok, oz);
             }
         }
-        __syncthreads();
+        // (no barrier: what the next tile's first part overwrites are the thread's own tokens, and the shares are not
+        // written before the barrier behind it)
     }
     const int64_t c = (int64_t)p.b * a.nchunk + p.chunk;
     if (ok) {
@@ -926,6 +935,15 @@ static int scan_prep(const Scan& a, int W, hipStream_t st) {
     return RST_OK;
 }
 
+template <bool REV>
+static int scan_chain(const Scan& a, int states, hipStream_t st) {
+    const dim3 grid((unsigned)cdiv(a.D, 64), states, a.B);
+    if (a.nchunk <= 32) hipLaunchKernelGGL((scan_chain_kernel<REV, 4>), grid, dim3(256), 0, st, a, states);
+    else hipLaunchKernelGGL((scan_chain_kernel<REV, 16>), grid, dim3(1024), 0, st, a, states);
+    RST_LAUNCH_CHECK();
+    return RST_OK;
+}
+
 template <typename T, int W, bool Z>
 static int scan_fwd_t(const Scan& a, hipStream_t st) {
     const double n = (double)a.B * a.D * a.L;
@@ -936,8 +954,7 @@ static int scan_fwd_t(const Scan& a, hipStream_t st) {
     if (a.nchunk > 1) {
         hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
         RST_LAUNCH_CHECK();
-        hipLaunchKernelGGL((scan_chain_kernel<false>), dim3((unsigned)cdiv(a.D, 64), 4 * W, a.B), dim3(1024), 0, st, a, 4 * W);
-        RST_LAUNCH_CHECK();
+        RST_TRY(scan_chain<false>(a, 4 * W, st));
     }
     hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a, a.bc);
     RST_LAUNCH_CHECK();
@@ -953,8 +970,7 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
     if (a.nchunk > 1) {
         hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
         RST_LAUNCH_CHECK();
-        hipLaunchKernelGGL((scan_chain_kernel<true>), dim3((unsigned)cdiv(a.D, 64), 4 * W, a.B), dim3(1024), 0, st, a, 4 * W);
-        RST_LAUNCH_CHECK();
+        RST_TRY(scan_chain<true>(a, 4 * W, st));
     }
     const size_t lds = (size_t)(3 + (Z ? 3 : 2) * W) * ST * SROW * sizeof(float);
     KernelSetup ks;
