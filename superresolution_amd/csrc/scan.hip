@@ -23,6 +23,8 @@
 // State, decay, sums and partial sums are fp32.
 #include "seq_common.hpp"
 
+#include <utility>
+
 namespace rst {
 
 constexpr int ST = 16;                 // tokens of a tile
@@ -123,6 +125,27 @@ template <int K> struct TokensBC {
     __device__ __forceinline__ float B(int j, int s) const { return v[j >> 1][(j & 1) * 8 + s]; }
     __device__ __forceinline__ float C(int j, int s) const { return v[j >> 1][(j & 1) * 8 + 4 + s]; }
 };
+// The rank-one updates of a wave's 64 channels x 4 states, state += (a token's B or C) x (a value a channel), are one matrix
+// instruction instead of four multiply-adds: v_mfma_f32_4x4x1 with 16 blocks of 4 states x 4 channels, whose result lies as
+// the states do (lane = channel, register = state).  Its first operand is broadcast from one block of four lanes, so ONE
+// register holds the 16 tokens x 4 states of a tile (lane 4 t + s: token t, state s).
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+template <int TOKEN> __device__ __forceinline__ void rank_one(float tile, float value, float (&h)[4]) {
+    const f32x4v c = {h[0], h[1], h[2], h[3]};
+    const f32x4v r = __builtin_amdgcn_mfma_f32_4x4x1f32(tile, value, c, 4, TOKEN, 0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) h[s] = r[s];
+}
+// the tile's B (at = 0) or C (at = 4) of the wave's states in that form
+__device__ __forceinline__ float tile_operand(const float* __restrict__ bc, int tile, int at, int lane) {
+    return (bc + (int64_t)tile * ST * 8)[(uint32_t)((lane >> 2) * 8 + (lane & 3) + at)];
+}
+// f(0), f(1), .. as constants (the token of a matrix instruction is part of it)
+template <int... I, typename F> __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void each(F&& f) { each_of(std::make_integer_sequence<int, N>{}, f); }
+
 // Scalar loads come back in any order, so a wait for one is a wait for all of them and for the LDS reads between.  The
 // token loops therefore go in groups: what the next group needs is asked for right behind a wait that has nothing
 // younger in it, and a group's work hides it (left to itself the compiler loads in front of each use: backward 1108
@@ -244,6 +267,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
         sum[k] = 0.f;
     }
     fetch(REV ? t1 - 1 : t0);
+    float vbn = tile_operand(bc, REV ? t1 - 1 : t0, REV ? 4 : 0, p.lane);
     for (int n = 0; n < t1 - t0; ++n) {
         const int tile = REV ? t1 - 1 - n : t0 + n;
         const ScanTile tl = scan_tile(a, p, tile);
@@ -265,36 +289,23 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
                 }
             }
         }
-        if (n + 1 < t1 - t0) fetch(REV ? tile - 1 : tile + 1);
-        __syncthreads();
-        TokensBC<4> v, vn;
-        float dt[4], u[4], dtn[4], un[4];
-        auto ask = [&](int g) {                                            // the g-th group on the way
-            const int j0 = (REV ? 3 - g : g) * 4;
-            vn.load(bc, (int64_t)tile * ST + j0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { dtn[j] = dts[j0 + j][p.lane]; un[j] = us[j0 + j][p.lane]; }
-        };
-        ask(0);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            group_arrived();
-            v = vn;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; }
-            if (g < 3) ask(g + 1);
-            group_asked();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = REV ? 3 - i : i;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const float decay = __builtin_amdgcn_exp2f(dt[j] * A[s]);
-                    if constexpr (REV) h[s] = decay * fmaf(u[j], v.C(j, s), h[s]);
-                    else h[s] = fmaf(decay, h[s], u[j] * v.B(j, s));
-                }
-            }
+        const float vb = vbn;
+        if (n + 1 < t1 - t0) {
+            fetch(REV ? tile - 1 : tile + 1);
+            vbn = tile_operand(bc, REV ? tile - 1 : tile + 1, REV ? 4 : 0, p.lane);
         }
+        __syncthreads();
+        each<ST>([&](auto I) {
+            constexpr int i = REV ? ST - 1 - I : I;
+            const float dt = dts[i][p.lane], u = us[i][p.lane];
+            float decay[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) decay[s] = __builtin_amdgcn_exp2f(dt * A[s]);
+            if constexpr (REV) rank_one<i>(vb, u, h);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) h[s] *= decay[s];
+            if constexpr (!REV) rank_one<i>(vb, u, h);
+        });
         __syncthreads();
     }
     const int64_t c = (int64_t)p.b * a.nchunk + p.chunk;
@@ -409,7 +420,9 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
         h[s] = start_state<W>(a, p, d, ok, s, a.h0);
     }
     const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
+    float vbn = tile_operand(bc, t0, 0, p.lane);
     for (int tile = t0; tile < t1; ++tile) {
+        const float vb = vbn;
         const ScanTile tl = scan_tile(a, p, tile);
         float x[NI][4], gate[NI][4];
 #pragma unroll
@@ -426,7 +439,10 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
                 }
             }
         }
-        if (tile + 1 < t1) fetch(tile + 1);
+        if (tile + 1 < t1) {
+            fetch(tile + 1);
+            vbn = tile_operand(bc, tile + 1, 0, p.lane);
+        }
         __syncthreads();
         if (a.ckpt && ok) {
 #pragma unroll
@@ -441,25 +457,25 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
             for (int j = 0; j < 4; ++j) { dtn[j] = dts[g * 4 + j][p.lane]; un[j] = us[g * 4 + j][p.lane]; }
         };
         ask(0);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        each<4>([&](auto G) {
+            constexpr int g = G;
             group_arrived();
             v = vn;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; }
-            if (g < 3) ask(g + 1);
+            if constexpr (g < 3) ask(g + 1);
             group_asked();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            each<4>([&](auto J) {
+                constexpr int j = J;
                 float y = 0.f;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    h[s] = fmaf(__builtin_amdgcn_exp2f(dt[j] * A[s]), h[s], u[j] * v.B(j, s));
-                    y = fmaf(v.C(j, s), h[s], y);
-                }
+                for (int s = 0; s < 4; ++s) h[s] *= __builtin_amdgcn_exp2f(dt[j] * A[s]);
+                rank_one<g * 4 + j>(vb, u[j], h);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) y = fmaf(v.C(j, s), h[s], y);
                 part[p.wave][g * 4 + j][p.lane] = y;
-            }
-        }
+            });
+        });
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
@@ -596,6 +612,7 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
         for (int s = 0; s < 4; ++s) hs[0][s] = ok ? hn[s] : 0.f;
         __syncthreads();
         const float* bct = bc + (int64_t)tile * ST * 8;
+        const float vb = tile_operand(bc, tile, 0, p.lane), vc = tile_operand(bc, tile, 4, p.lane);
         TokensBC<2> v, vn;
         float dt[2], u[2], e[2], dtn[2], un[2], en[2];
         auto ask = [&](int j0, bool with_e) {                              // tokens j0 and j0 + 1 on the way
@@ -614,43 +631,41 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
             for (int j = 0; j < 2; ++j) { dt[j] = dtn[j]; u[j] = un[j]; e[j] = en[j]; }
         };
         ask(0, false);
-#pragma unroll
-        for (int i0 = 0; i0 < ST; i0 += 2) {
+        each<ST / 2>([&](auto G) {
+            constexpr int i0 = 2 * G;
             take();
-            if (i0 + 2 < ST) ask(i0 + 2, false);
-            else {
-                // (the way back reads B and C again: the compiler would rather keep all of them, in lanes of vector registers)
-                
-                ask(ST - 2, true);
-            }
+            if constexpr (i0 + 2 < ST) ask(i0 + 2, false);
+            else ask(ST - 2, true);
             group_asked();
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = i0 + j;
+            each<2>([&](auto J) {
+                constexpr int j = J, i = i0 + j;
                 float y = 0.f;
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     as[i][s] = __builtin_amdgcn_exp2f(dt[j] * A2[s]);
-                    hs[i + 1][s] = fmaf(as[i][s], hs[i][s], u[j] * v.B(j, s));
-                    if constexpr (Z) y = fmaf(v.C(j, s), hs[i + 1][s], y);
+                    hs[i + 1][s] = as[i][s] * hs[i][s];
                 }
-                if constexpr (Z) part2[p.wave][i][p.lane] = y;
-            }
-        }
-        float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
+                rank_one<i>(vb, u[j], hs[i + 1]);
+                if constexpr (Z) {
 #pragma unroll
-        for (int i0 = ST - 2; i0 >= 0; i0 -= 2) {
+                    for (int s = 0; s < 4; ++s) y = fmaf(v.C(j, s), hs[i + 1][s], y);
+                    part2[p.wave][i][p.lane] = y;
+                }
+            });
+        });
+        float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
+        each<ST / 2>([&](auto G) {
+            constexpr int i0 = ST - 2 - 2 * G;
             take();
-            if (i0 > 0) ask(i0 - 2, true);
+            if constexpr (i0 > 0) ask(i0 - 2, true);
             if (i0 == ST / 2 - 2 && tile > t0) fetch(tile - 1);            // (half of the states are done with: registers are free)
             group_asked();
-#pragma unroll
-            for (int j = 1; j >= 0; --j) {
-                const int i = i0 + j;
+            each<2>([&](auto J) {
+                constexpr int j = 1 - J, i = i0 + j;
                 float gB = 0.f, gA = 0.f, pr[8];
+                rank_one<i>(vc, e[j], g);
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    g[s] = fmaf(v.C(j, s), e[j], g[s]);
                     pr[s] = g[s] * u[j];
                     pr[4 + s] = hs[i + 1][s] * e[j];
                     gB = fmaf(g[s], v.B(j, s), gB);
@@ -667,8 +682,8 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
                 }
                 fold[i & 7] = lanes_fold(pr, p.lane);
                 if ((i & 7) == 0) (bco + ((int64_t)tile * 2 + (i >> 3)) * W * 64)[(uint32_t)p.lane] = tokens_fold(fold, p.lane);
-            }
-        }
+            });
+        });
 #pragma unroll
         for (int s = 0; s < 4; ++s) dA[s] += tA[s];
         __syncthreads();
