@@ -234,7 +234,7 @@ __device__ __forceinline__ float gate_of(const Quad<T>& z, int i) {
 
 // ---- what a chunk adds to the state behind it (REV: to the state's gradient before it), and the sum of its dt -------
 template <typename T, int W, bool Z, bool REV>
-__global__ void __launch_bounds__(64 * W)
+__global__ void __launch_bounds__(64 * W, 8)                               // (at most 256 registers: else the matrix results go to AGPRs and back)
 scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
     constexpr int NI = ScanItems<W>::N;
     __shared__ float dts[ST][SROW], us[ST][SROW];
@@ -746,7 +746,7 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
 }
 
 template <typename T, int W, bool Z>
-__global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)
+__global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)                  // (fewer waves have more tokens a lane: 256 registers would spill)
 scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
     extern __shared__ __attribute__((aligned(16))) float smem[];
     const ScanPlace p(a, a.nchunk, 0);
