@@ -323,9 +323,9 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 
 // ---- the chunks' own states, one behind the other: cst[c] becomes the state that chunk c starts from (REV: the
 // state's gradient behind it).  A block has 64 channels and one state; its waves take a run of chunks each, side by side,
-// chain the runs through LDS and walk their run again: four waves for up to 32 chunks, which then stay in registers, else 16.  (Chained in front of every chunk by the scan's own blocks, the
+// chain the runs through LDS and walk their run again: four waves with up to 8 chunks each, or 16 with 16; what a run of that length reads stays in registers for the second walk.  (Chained in front of every chunk by the scan's own blocks, the
 // states are read as often as there are chunks: 503 MB from the caches for 256 chunks of 192 channels, 45 us instead of 20.)
-template <bool REV, int RUNS>
+template <bool REV, int RUNS, int LEN>
 __global__ void __launch_bounds__(64 * RUNS)
 scan_chain_kernel(const Scan a, int states) {
     __shared__ float sums[RUNS][64], own[RUNS][64];
@@ -345,12 +345,12 @@ scan_chain_kernel(const Scan a, int states) {
         v = st[k * states * a.D + dr];
         if (!in) { t = 0.f; v = 0.f; }
     };
-    float sum = 0.f, h = 0.f, t[8], v[8];
-    for (int c = c0; c < c1; c += 8) {
+    float sum = 0.f, h = 0.f, t[LEN], v[LEN];
+    for (int c = c0; c < c1; c += LEN) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) read(c + j, t[j], v[j]);
+        for (int j = 0; j < LEN; ++j) read(c + j, t[j], v[j]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < LEN; ++j) {
             sum += t[j];
             h = fmaf(__builtin_amdgcn_exp2f(t[j] * A), h, v[j]);
         }
@@ -361,13 +361,13 @@ scan_chain_kernel(const Scan a, int states) {
     const float* first = REV ? a.dlast : a.h0;
     h = first && n < a.N ? first[((int64_t)b * a.D + dr) * a.N + n] : 0.f;
     for (int r = 0; r < run; ++r) h = fmaf(__builtin_amdgcn_exp2f(sums[r][lane] * A), h, own[r][lane]);
-    for (int c = c0; c < c1; c += 8) {
-        if (c1 - c0 > 8) {                                                 // (a run of at most eight is still in registers)
+    for (int c = c0; c < c1; c += LEN) {
+        if (c1 - c0 > LEN) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) read(c + j, t[j], v[j]);
+            for (int j = 0; j < LEN; ++j) read(c + j, t[j], v[j]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < LEN; ++j)
             if (c + j < c1) {
                 const int64_t k = REV ? a.nchunk - 1 - (c + j) : c + j;
                 if (ok) st[k * states * a.D + d] = h;
@@ -953,8 +953,8 @@ static int scan_prep(const Scan& a, int W, hipStream_t st) {
 template <bool REV>
 static int scan_chain(const Scan& a, int states, hipStream_t st) {
     const dim3 grid((unsigned)cdiv(a.D, 64), states, a.B);
-    if (a.nchunk <= 32) hipLaunchKernelGGL((scan_chain_kernel<REV, 4>), grid, dim3(256), 0, st, a, states);
-    else hipLaunchKernelGGL((scan_chain_kernel<REV, 16>), grid, dim3(1024), 0, st, a, states);
+    if (a.nchunk <= 32) hipLaunchKernelGGL((scan_chain_kernel<REV, 4, 8>), grid, dim3(256), 0, st, a, states);
+    else hipLaunchKernelGGL((scan_chain_kernel<REV, 16, 16>), grid, dim3(1024), 0, st, a, states);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
