@@ -10,8 +10,9 @@
 // Bound by the vector pipe, not by memory: one exponential and five more operations per state and token forward (16
 // states: 96 operations for the 6 to 12 bytes of a bf16 or fp32 token), so the layout serves the instruction stream:
 //   - a lane is a channel and holds four of its states; the waves of a block hold the other states of the same 64
-//     channels.  B and C are then the same for a whole wave and come in as scalar operands (no vector register, no LDS).
-//     They are laid out for that once per call: [B][G][wave][token][B0..B3 C0..C3] in fp32 (bc_prep_kernel).
+//     channels.  B and C are then the same for a whole wave: scalar operands of multiply-adds (TokensBC), or the broadcast
+//     operand of the matrix instruction that adds a token's input to 64 x 4 states (rank_one).  They are laid out for that
+//     once per call: [B][G][wave][token][B0..B3 C0..C3] in fp32 (bc_prep_kernel).
 //   - tokens go in tiles of 16.  The tensors are token-contiguous, so a thread loads 4 tokens of one channel (a wave: 16
 //     channels x 16 tokens), takes softplus once, and hands dt and dt x over through LDS, turned to lane = channel; the
 //     waves' shares of s come back the same way.
@@ -147,7 +148,7 @@ template <int... I, typename F> __device__ __forceinline__ void each_of(std::int
 template <int N, typename F> __device__ __forceinline__ void each(F&& f) { each_of(std::make_integer_sequence<int, N>{}, f); }
 
 // Scalar loads come back in any order, so a wait for one is a wait for all of them and for the LDS reads between.  The
-// token loops therefore go in groups: what the next group needs is asked for right behind a wait that has nothing
+// token loops that read them go in groups: what the next group needs is asked for right behind a wait that has nothing
 // younger in it, and a group's work hides it (left to itself the compiler loads in front of each use: backward 1108
 // against 887 us).  Four tokens a group; two backward, whose token is four times the work and whose scalar registers
 // would spill to lanes of vector registers.
@@ -323,8 +324,13 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 
 // ---- the chunks' own states, one behind the other: cst[c] becomes the state that chunk c starts from (REV: the
 // state's gradient behind it).  A block has 64 channels and one state; its waves take a run of chunks each, side by side,
-// chain the runs through LDS and walk their run again: four waves with up to 8 chunks each, or 16 with 16; what a run of that length reads stays in registers for the second walk.  (Chained in front of every chunk by the scan's own blocks, the
+// chain the runs through LDS and walk their run again: four waves with up to 8 chunks each, or 16 with 16; what a run of that
+// length reads stays in registers for the second walk.  (Chained in front of every chunk by the scan's own blocks, the
 // states are read as often as there are chunks: 503 MB from the caches for 256 chunks of 192 channels, 45 us instead of 20.)
+// A state of zero stays zero over a chunk whose decay overflows (growing states, A > 0): 0 times infinity is no number.
+__device__ __forceinline__ float over_chunk(float h, float sum, float A, float own) {
+    return h == 0.f ? own : fmaf(__builtin_amdgcn_exp2f(sum * A), h, own);
+}
 template <bool REV, int RUNS, int LEN>
 __global__ void __launch_bounds__(64 * RUNS)
 scan_chain_kernel(const Scan a, int states) {
@@ -352,7 +358,7 @@ scan_chain_kernel(const Scan a, int states) {
 #pragma unroll
         for (int j = 0; j < LEN; ++j) {
             sum += t[j];
-            h = fmaf(__builtin_amdgcn_exp2f(t[j] * A), h, v[j]);
+            h = over_chunk(h, t[j], A, v[j]);
         }
     }
     sums[run][lane] = sum;
@@ -360,7 +366,7 @@ scan_chain_kernel(const Scan a, int states) {
     __syncthreads();
     const float* first = REV ? a.dlast : a.h0;
     h = first && n < a.N ? first[((int64_t)b * a.D + dr) * a.N + n] : 0.f;
-    for (int r = 0; r < run; ++r) h = fmaf(__builtin_amdgcn_exp2f(sums[r][lane] * A), h, own[r][lane]);
+    for (int r = 0; r < run; ++r) h = over_chunk(h, sums[r][lane], A, own[r][lane]);
     for (int c = c0; c < c1; c += LEN) {
         if (c1 - c0 > LEN) {
 #pragma unroll
@@ -371,7 +377,7 @@ scan_chain_kernel(const Scan a, int states) {
             if (c + j < c1) {
                 const int64_t k = REV ? a.nchunk - 1 - (c + j) : c + j;
                 if (ok) st[k * states * a.D + d] = h;
-                h = fmaf(__builtin_amdgcn_exp2f(t[j] * A), h, v[j]);
+                h = over_chunk(h, t[j], A, v[j]);
             }
     }
 }

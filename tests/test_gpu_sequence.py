@@ -302,6 +302,23 @@ def test_selective_scan_infinite_values_stay_in_their_channel():
     assert torch.isfinite(dev["C"].grad).all()
 
 
+def test_selective_scan_growing_states():
+    """Rates above zero: a state of zero stays zero over chunks whose growth does not fit fp32, and grows from there."""
+    g = _gen(14)
+    c = _scan_case(g, 1, 5, 1, 4, 900, F32, False, False, False)
+    c["A"], c["delta"] = -c["A"], torch.full_like(c["delta"], 0.5)
+    c["x"][..., :880] = 0
+    c["C"][..., 20:] = 0                                   # the gradient of the states behind is zero too, from the other end
+    dev = {k: _leaf(v) for k, v in c.items()}
+    y, last = sequence.selective_scan(*_scan_args(dev), return_last_state=True)
+    assert not y.any()
+    cut = {k: (v[..., 880:] if k in ("x", "delta", "B", "C") else v) for k, v in c.items()}
+    want, mag = so.scan(*_scan_args(cut))
+    so.within(last, want["last"], mag["last"], 400, "last")
+    y.sum().backward()
+    assert all(torch.isfinite(v.grad).all() for k, v in dev.items() if v is not None and k != "h0")
+
+
 def test_empty_sequences():
     w, A = torch.randn(4, 3, device="cuda"), -torch.rand(4, 5, device="cuda")
     for B, L in ((2, 0), (0, 6)):
