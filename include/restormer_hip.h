@@ -613,8 +613,9 @@ typedef struct rst_scan_grads {
     float* delta_bias;
 } rst_scan_grads;
 /* state_in, state_out: or NULL.  saved: rst_scan_saved_bytes for a backward    */
-/* pass (the states every 16 tokens; B and C in fp32), or NULL.  L <= 2^24.      */
-/* Workspaces and saved are aligned to 256 bytes.                                */
+/* pass (the states every 16 tokens), or NULL.  L <= 2^24.  Workspaces are        */
+/* aligned to 16 bytes; the forward pass needs none (0 bytes) where the chip is     */
+/* full without cutting the tokens into chunks.                                   */
 size_t rst_scan_workspace_bytes(const rst_scan_desc* desc);
 size_t rst_scan_saved_bytes(const rst_scan_desc* desc);
 int rst_scan_fwd(const rst_scan_desc* desc, const rst_scan_inputs* inputs, const float* state_in, void* y,

@@ -10,9 +10,8 @@
 // Bound by the vector pipe, not by memory: one exponential and five more operations per state and token forward (16
 // states: 96 operations for the 6 to 12 bytes of a bf16 or fp32 token), so the layout serves the instruction stream:
 //   - a lane is a channel and holds four of its states; the waves of a block hold the other states of the same 64
-//     channels.  B and C are then the same for a whole wave: scalar operands of multiply-adds (TokensBC), or the broadcast
-//     operand of the matrix instruction that adds a token's input to 64 x 4 states (rank_one).  They are laid out for that
-//     once per call: [B][G][wave][token][B0..B3 C0..C3] in fp32 (bc_prep_kernel).
+//     channels.  B and C are then the same for a whole wave: one register holds its share of a tile and is the broadcast
+//     operand of the matrix instruction that adds a token's input to 64 x 4 states (rank_one); LDS has it for the sums.
 //   - tokens go in tiles of 16.  The tensors are token-contiguous, so a thread loads 4 tokens of one channel (a wave: 16
 //     channels x 16 tokens), takes softplus once, and hands dt and dt x over through LDS, turned to lane = channel; the
 //     waves' shares of s come back the same way.
@@ -30,14 +29,13 @@ namespace rst {
 
 constexpr int ST = 16;                 // tokens of a tile
 constexpr int SC = 64;                 // channels of a block
-constexpr int SROW = 68;               // LDS row of a token: 64 channels, padded so that 4 tokens apart is 16 banks apart
+constexpr int SROW = 68;               // LDS row of a token: 64 channels and four more, so that 4 tokens apart is 16 banks apart
 
 struct Scan {
     const void *x, *delta, *Bm, *Cm, *z, *dy;
     const float *A, *Dskip, *dbias, *h0, *dlast;
     void *y, *dx, *ddelta, *dB, *dC, *dz;
     float *last, *dh0;
-    float* bc;                          // [B][G][W][tiles * 16][8]
     float* ckpt;                        // [B][tiles][4 W][D]: the state at every tile's start, or null
     float* cst;                         // [B][chunks][4 W][D]: what a chunk adds to the state behind (backward: before) it
     float* cdt;                         // [B][chunks][D]: sum of dt
@@ -114,18 +112,6 @@ template <typename T> struct Quad {
     }
 };
 
-// B and C of K (2 or 4) tokens and a wave's four states, in scalar registers
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-template <int K> struct TokensBC {
-    f32x16 v[K / 2];
-    __device__ __forceinline__ void load(const float* __restrict__ bc, int64_t t) {
-        const f32x16* p = reinterpret_cast<const f32x16*>(bc + t * 8);
-#pragma unroll
-        for (int i = 0; i < K / 2; ++i) v[i] = p[i];
-    }
-    __device__ __forceinline__ float B(int j, int s) const { return v[j >> 1][(j & 1) * 8 + s]; }
-    __device__ __forceinline__ float C(int j, int s) const { return v[j >> 1][(j & 1) * 8 + 4 + s]; }
-};
 // The rank-one updates of a wave's 64 channels x 4 states, state += (a token's B or C) x (a value a channel), are one matrix
 // instruction instead of four multiply-adds: v_mfma_f32_4x4x1 with 16 blocks of 4 states x 4 channels, whose result lies as
 // the states do (lane = channel, register = state).  Its first operand is broadcast from one block of four lanes, so ONE
@@ -137,27 +123,39 @@ template <int TOKEN> __device__ __forceinline__ void rank_one(float tile, float 
 #pragma unroll
     for (int s = 0; s < 4; ++s) h[s] = r[s];
 }
-// the tile's B (at = 0) or C (at = 4) of the wave's states in that form
-__device__ __forceinline__ float tile_operand(const float* __restrict__ bc, int tile, int at, int lane) {
-    return (bc + (int64_t)tile * ST * 8)[(uint32_t)((lane >> 2) * 8 + (lane & 3) + at)];
+// A wave's share of B or C at a tile in that form: token lane / 4, state 4 wave + lane % 4, zero behind the last state or token.
+// The loads touch four rows of 16 tokens.  (31 rows of 2^24 values are the furthest offset: below 2^31 bytes.)
+template <typename T> struct TileOperand {
+    const T* base; uint32_t row; int t; bool in;
+    __device__ __forceinline__ TileOperand(const void* m, const Scan& a, int64_t bg, int wave, int lane) {
+        const int n = wave * 4 + (lane & 3);
+        in = n < a.N;
+        base = static_cast<const T*>(m) + bg * a.N * a.L;
+        row = in ? (uint32_t)n * (uint32_t)a.L : 0u;
+        t = lane >> 2;
+    }
+    __device__ __forceinline__ float load(int tile, int left) const {
+        const char* p = reinterpret_cast<const char*>(base + (int64_t)tile * ST);
+        const float v = Store<T>::get(*reinterpret_cast<const T*>(p + (row + (t < left ? t : left - 1)) * (uint32_t)sizeof(T)));
+        return in && t < left ? v : 0.f;
+    }
+};
+// Where a state's B or C multiplies a sum of its own instead, the wave reads the four of a token back from LDS, one
+// 16-byte read at the same address for all lanes.  (As scalar loads from a copy laid out for it they came back in any order: a
+// wait for one was a wait for all and for the LDS reads between, and the copy was a launch of its own.)
+// The four stand in the padding of the token's row of the wave's shares: 1 KiB more of LDS would cost the forward kernel a
+// block a compute unit (262 -> 302 us).
+struct Four { float v[4]; };
+__device__ __forceinline__ void keep_fours(float (&rows)[ST][SROW], int lane, float operand) { rows[lane >> 2][SC + (lane & 3)] = operand; }
+__device__ __forceinline__ Four four_at(const float (&rows)[ST][SROW], int token) {
+    const f32x4v q = *reinterpret_cast<const f32x4v*>(&rows[token][SC]);
+    return {{q[0], q[1], q[2], q[3]}};
 }
 // f(0), f(1), .. as constants (the token of a matrix instruction is part of it)
 template <int... I, typename F> __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
     (f(std::integral_constant<int, I>{}), ...);
 }
 template <int N, typename F> __device__ __forceinline__ void each(F&& f) { each_of(std::make_integer_sequence<int, N>{}, f); }
-
-// Scalar loads come back in any order, so a wait for one is a wait for all of them and for the LDS reads between.  The
-// token loops that read them go in groups: what the next group needs is asked for right behind a wait that has nothing
-// younger in it, and a group's work hides it (left to itself the compiler loads in front of each use: backward 1108
-// against 887 us).  Four tokens a group; two backward, whose token is four times the work and whose scalar registers
-// would spill to lanes of vector registers.
-__device__ __forceinline__ void group_arrived() {
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0xC07F);                                    // lgkmcnt(0)
-    __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ void group_asked() { __builtin_amdgcn_sched_barrier(0); }
 
 // a block of W waves has 64 channels x 4 quads of a tile to load: items per thread
 template <int W> struct ScanItems { static constexpr int N = W >= 4 ? 1 : 4 / W; };
@@ -182,29 +180,6 @@ __device__ __forceinline__ ScanTile scan_tile(const Scan& a, const ScanPlace& p,
 }
 
 __device__ __forceinline__ float step_size(const Scan& a, float raw) { return a.softplus ? softplus(raw) : raw; }
-
-// B and C as the scan's waves read them: [b][g][wave][token][B0..B3 C0..C3], zeros behind the last state and token.
-// Threads run along the tokens, so the reads are whole lines.
-template <typename T>
-__global__ void __launch_bounds__(256)
-bc_prep_kernel(const T* __restrict__ Bm, const T* __restrict__ Cm, float* __restrict__ bc, int N, int W, int64_t L, int64_t Lp) {
-    const int64_t t = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int64_t bg = blockIdx.y;
-    if (t >= Lp) return;
-    for (int w = threadIdx.x >> 6; w < W; w += 4) {
-        float v[8];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int n = w * 4 + s;
-            const bool in = n < N && t < L;
-            v[s] = in ? Store<T>::get(Bm[(bg * N + n) * L + t]) : 0.f;
-            v[4 + s] = in ? Store<T>::get(Cm[(bg * N + n) * L + t]) : 0.f;
-        }
-        Raw<float, 8> o;
-        o.pack(v);
-        o.store(bc + ((bg * W + w) * Lp + t) * 8);
-    }
-}
 
 // A (times log2 e) of the lane's channel and four states; zero where there are none, so that they stay zero
 __device__ __forceinline__ void load_rates(const Scan& a, int d, bool ok, int wave, float (&A)[4]) {
@@ -236,7 +211,7 @@ __device__ __forceinline__ float gate_of(const Quad<T>& z, int i) {
 // ---- what a chunk adds to the state behind it (REV: to the state's gradient before it), and the sum of its dt -------
 template <typename T, int W, bool Z, bool REV>
 __global__ void __launch_bounds__(64 * W, 8)                               // (at most 256 registers: else the matrix results go to AGPRs and back)
-scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
+scan_chunk_kernel(const Scan a) {
     constexpr int NI = ScanItems<W>::N;
     __shared__ float dts[ST][SROW], us[ST][SROW];
     const ScanPlace p(a, a.nchunk - 1, REV ? 1 : 0);
@@ -248,12 +223,13 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) A[s] *= LOG2E;
     const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
-    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
+    const TileOperand<T> op(REV ? a.Cm : a.Bm, a, (int64_t)p.b * a.G + p.g, p.wave, p.lane);
     ScanItem<W> it[NI];
-    float bias[NI];
+    float bias[NI], vbn;
     Quad<T> qd[NI], qx[NI], qz[NI];
     auto fetch = [&](int tile) {
         const ScanTile tl = scan_tile(a, p, tile);
+        vbn = op.load(tile, tl.left);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             qd[k].load(a.delta, tl, it[k].row, it[k].q);
@@ -268,7 +244,6 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
         sum[k] = 0.f;
     }
     fetch(REV ? t1 - 1 : t0);
-    float vbn = tile_operand(bc, REV ? t1 - 1 : t0, REV ? 4 : 0, p.lane);
     for (int n = 0; n < t1 - t0; ++n) {
         const int tile = REV ? t1 - 1 - n : t0 + n;
         const ScanTile tl = scan_tile(a, p, tile);
@@ -291,10 +266,7 @@ scan_chunk_kernel(const Scan a, const float* __restrict__ bc0) {
             }
         }
         const float vb = vbn;
-        if (n + 1 < t1 - t0) {
-            fetch(REV ? tile - 1 : tile + 1);
-            vbn = tile_operand(bc, REV ? tile - 1 : tile + 1, REV ? 4 : 0, p.lane);
-        }
+        if (n + 1 < t1 - t0) fetch(REV ? tile - 1 : tile + 1);
         __syncthreads();
         each<ST>([&](auto I) {
             constexpr int i = REV ? ST - 1 - I : I;
@@ -392,18 +364,22 @@ __device__ __forceinline__ float start_state(const Scan& a, const ScanPlace& p, 
 // ---- forward ------------------------------------------------------------------------------------------------------
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, 6)
-scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
+scan_fwd_kernel(const Scan a) {
     constexpr int NI = ScanItems<W>::N;
-    __shared__ float dts[ST][SROW], us[ST][SROW], part[W][ST][SROW];
+    __shared__ __attribute__((aligned(16))) float dts[ST][SROW], us[ST][SROW], part[W][ST][SROW];
     const ScanPlace p(a, a.nchunk, 0);
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
     const bool ok = p.cb * SC + p.lane < a.Dg, whole = p.cb * SC + SC <= a.Dg;
+    const int64_t bg = (int64_t)p.b * a.G + p.g;
+    const TileOperand<T> opb(a.Bm, a, bg, p.wave, p.lane), opc(a.Cm, a, bg, p.wave, p.lane);
     const int t0 = p.chunk * a.per_chunk, t1 = t0 + a.per_chunk < a.tiles ? t0 + a.per_chunk : a.tiles;
     ScanItem<W> it[NI];
-    float bias[NI], skip[NI];
+    float bias[NI], skip[NI], vbn, vcn;
     Quad<T> qd[NI], qx[NI], qz[NI];
     auto fetch = [&](int tile) {
         const ScanTile tl = scan_tile(a, p, tile);
+        vbn = opb.load(tile, tl.left);
+        vcn = opc.load(tile, tl.left);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             qd[k].load(a.delta, tl, it[k].row, it[k].q);
@@ -425,8 +401,6 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
         A[s] *= LOG2E;
         h[s] = start_state<W>(a, p, d, ok, s, a.h0);
     }
-    const float* bc = bc0 + ((int64_t)(p.b * a.G + p.g) * W + p.wave) * a.tiles * ST * 8;
-    float vbn = tile_operand(bc, t0, 0, p.lane);
     for (int tile = t0; tile < t1; ++tile) {
         const float vb = vbn;
         const ScanTile tl = scan_tile(a, p, tile);
@@ -445,42 +419,25 @@ scan_fwd_kernel(const Scan a, const float* __restrict__ bc0) {
                 }
             }
         }
-        if (tile + 1 < t1) {
-            fetch(tile + 1);
-            vbn = tile_operand(bc, tile + 1, 0, p.lane);
-        }
+        keep_fours(part[p.wave], p.lane, vcn);
+        if (tile + 1 < t1) fetch(tile + 1);
         __syncthreads();
         if (a.ckpt && ok) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 (a.ckpt + (((int64_t)p.b * a.tiles + tile) * 4 * W + p.wave * 4 + s) * a.D)[(uint32_t)d] = h[s];
         }
-        TokensBC<4> v, vn;
-        float dt[4], u[4], dtn[4], un[4];
-        auto ask = [&](int g) {                                            // the g-th group on the way
-            vn.load(bc, (int64_t)tile * ST + g * 4);
+        each<ST>([&](auto I) {
+            constexpr int i = I;
+            const float dt = dts[i][p.lane], u = us[i][p.lane];
+            const Four cv = four_at(part[p.wave], i);
+            float y = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { dtn[j] = dts[g * 4 + j][p.lane]; un[j] = us[g * 4 + j][p.lane]; }
-        };
-        ask(0);
-        each<4>([&](auto G) {
-            constexpr int g = G;
-            group_arrived();
-            v = vn;
+            for (int s = 0; s < 4; ++s) h[s] *= __builtin_amdgcn_exp2f(dt * A[s]);
+            rank_one<i>(vb, u, h);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { dt[j] = dtn[j]; u[j] = un[j]; }
-            if constexpr (g < 3) ask(g + 1);
-            group_asked();
-            each<4>([&](auto J) {
-                constexpr int j = J;
-                float y = 0.f;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) h[s] *= __builtin_amdgcn_exp2f(dt[j] * A[s]);
-                rank_one<g * 4 + j>(vb, u[j], h);
-#pragma unroll
-                for (int s = 0; s < 4; ++s) y = fmaf(v.C(j, s), h[s], y);
-                part[p.wave][g * 4 + j][p.lane] = y;
-            });
+            for (int s = 0; s < 4; ++s) y = fmaf(cv.v[s], h[s], y);
+            part[p.wave][i][p.lane] = y;
         });
         __syncthreads();
 #pragma unroll
@@ -543,7 +500,7 @@ __device__ __forceinline__ float tokens_fold(const float (&w)[8], int lane) {
 // WHOLE: the block has 64 channels.  Where it has fewer, the shares of the lanes without one are taken out: they are
 // zero only as long as B and C are finite.
 template <typename T, int W, bool Z, bool WHOLE>
-__device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __restrict__ bc0, const ScanPlace& p, float* smem) {
+__device__ __forceinline__ void scan_bwd_body(const Scan& a, const ScanPlace& p, float* smem) {
     constexpr int NI = ScanItems<W>::N;
     float (*dts)[SROW] = reinterpret_cast<float (*)[SROW]>(smem);
     float (*us)[SROW] = dts + ST;
@@ -566,9 +523,13 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
         db[k] = 0.f;
     }
     Quad<T> qd[NI], qx[NI], qy[NI], qz[NI];
-    float hn[4];
+    float hn[4], vbn, vcn;
+    const int64_t bg = (int64_t)p.b * a.G + p.g;
+    const TileOperand<T> opb(a.Bm, a, bg, p.wave, p.lane), opc(a.Cm, a, bg, p.wave, p.lane);
     auto fetch = [&](int tile) {
         const ScanTile tl = scan_tile(a, p, tile);
+        vbn = opb.load(tile, tl.left);
+        vcn = opc.load(tile, tl.left);
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             qd[k].load(a.delta, tl, it[k].row, it[k].q);
@@ -587,8 +548,6 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
         A2[s] = A[s] * LOG2E;
         g[s] = start_state<W>(a, p, d, ok, s, a.dlast);
     }
-    const int64_t bg = (int64_t)p.b * a.G + p.g;
-    const float* bc = bc0 + (bg * W + p.wave) * a.tiles * ST * 8;
     float* bco = a.bcpart + (((int64_t)p.cb * a.B * a.G + bg) * a.tiles * 2 * W + p.wave) * 64;
     for (int tile = t1 - 1; tile >= t0; --tile) {
         const ScanTile tl = scan_tile(a, p, tile);
@@ -616,79 +575,66 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
         float hs[ST + 1][4], as[ST][4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) hs[0][s] = ok ? hn[s] : 0.f;
+        const float vb = vbn, vc = vcn;
+        keep_fours(part0[p.wave], p.lane, vb);
+        if constexpr (Z) keep_fours(part1[p.wave], p.lane, vc);
         __syncthreads();
-        const float* bct = bc + (int64_t)tile * ST * 8;
-        const float vb = tile_operand(bc, tile, 0, p.lane), vc = tile_operand(bc, tile, 4, p.lane);
-        TokensBC<2> v, vn;
-        float dt[2], u[2], e[2], dtn[2], un[2], en[2];
-        auto ask = [&](int j0, bool with_e) {                              // tokens j0 and j0 + 1 on the way
-            vn.load(bct, j0);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                dtn[j] = dts[j0 + j][p.lane];
-                un[j] = us[j0 + j][p.lane];
-                if (with_e) en[j] = es[j0 + j][p.lane];
-            }
+        // the operands of the next token are read while one is worked on: two waves a SIMD do not hide the reads
+        float dt, u, e, dtn, un, en;
+        Four m, mn;
+        auto ask = [&](int i, bool back) {
+            dtn = dts[i][p.lane];
+            un = us[i][p.lane];
+            if (back) { en = es[i][p.lane]; mn = four_at(part0[p.wave], i); }
+            else if constexpr (Z) mn = four_at(part1[p.wave], i);
         };
-        auto take = [&]() {
-            group_arrived();
-            v = vn;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) { dt[j] = dtn[j]; u[j] = un[j]; e[j] = en[j]; }
-        };
+        auto take = [&]() { dt = dtn; u = un; e = en; m = mn; };
         ask(0, false);
-        each<ST / 2>([&](auto G) {
-            constexpr int i0 = 2 * G;
+        each<ST>([&](auto I) {
+            constexpr int i = I;
             take();
-            if constexpr (i0 + 2 < ST) ask(i0 + 2, false);
-            else ask(ST - 2, true);
-            group_asked();
-            each<2>([&](auto J) {
-                constexpr int j = J, i = i0 + j;
-                float y = 0.f;
+            ask(i + 1 < ST ? i + 1 : ST - 1, i + 1 == ST);
+            __builtin_amdgcn_sched_barrier(0);
+            float y = 0.f;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    as[i][s] = __builtin_amdgcn_exp2f(dt[j] * A2[s]);
-                    hs[i + 1][s] = as[i][s] * hs[i][s];
-                }
-                rank_one<i>(vb, u[j], hs[i + 1]);
-                if constexpr (Z) {
+            for (int s = 0; s < 4; ++s) {
+                as[i][s] = __builtin_amdgcn_exp2f(dt * A2[s]);
+                hs[i + 1][s] = as[i][s] * hs[i][s];
+            }
+            rank_one<i>(vb, u, hs[i + 1]);
+            if constexpr (Z) {
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) y = fmaf(v.C(j, s), hs[i + 1][s], y);
-                    part2[p.wave][i][p.lane] = y;
-                }
-            });
+                for (int s = 0; s < 4; ++s) y = fmaf(m.v[s], hs[i + 1][s], y);
+                part2[p.wave][i][p.lane] = y;
+            }
         });
         float tA[4] = {0.f, 0.f, 0.f, 0.f}, fold[8];
-        each<ST / 2>([&](auto G) {
-            constexpr int i0 = ST - 2 - 2 * G;
+        each<ST>([&](auto I) {
+            constexpr int i = ST - 1 - I;
             take();
-            if constexpr (i0 > 0) ask(i0 - 2, true);
-            if (i0 == ST / 2 - 2 && tile > t0) fetch(tile - 1);            // (half of the states are done with: registers are free)
-            group_asked();
-            each<2>([&](auto J) {
-                constexpr int j = 1 - J, i = i0 + j;
-                float gB = 0.f, gA = 0.f, pr[8];
-                rank_one<i>(vc, e[j], g);
+            if constexpr (i > 0) ask(i - 1, true);
+            if (i == ST / 2 && tile > t0) fetch(tile - 1);                 // (half of the states are done with: registers are free)
+            __builtin_amdgcn_sched_barrier(0);
+            float gB = 0.f, gA = 0.f, pr[8];
+            rank_one<i>(vc, e, g);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    pr[s] = g[s] * u[j];
-                    pr[4 + s] = hs[i + 1][s] * e[j];
-                    gB = fmaf(g[s], v.B(j, s), gB);
-                    g[s] *= as[i][s];
-                    const float q = g[s] * hs[i][s];
-                    gA = fmaf(A[s], q, gA);
-                    tA[s] = fmaf(dt[j], q, tA[s]);
-                }
-                part0[p.wave][i][p.lane] = gB;
-                part1[p.wave][i][p.lane] = gA;
-                if constexpr (!WHOLE) {
+            for (int s = 0; s < 4; ++s) {
+                pr[s] = g[s] * u;
+                pr[4 + s] = hs[i + 1][s] * e;
+                gB = fmaf(g[s], m.v[s], gB);
+                g[s] *= as[i][s];
+                const float q = g[s] * hs[i][s];
+                gA = fmaf(A[s], q, gA);
+                tA[s] = fmaf(dt, q, tA[s]);
+            }
+            part0[p.wave][i][p.lane] = gB;
+            part1[p.wave][i][p.lane] = gA;
+            if constexpr (!WHOLE) {
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) pr[s] = ok ? pr[s] : 0.f;
-                }
-                fold[i & 7] = lanes_fold(pr, p.lane);
-                if ((i & 7) == 0) (bco + ((int64_t)tile * 2 + (i >> 3)) * W * 64)[(uint32_t)p.lane] = tokens_fold(fold, p.lane);
-            });
+                for (int s = 0; s < 8; ++s) pr[s] = ok ? pr[s] : 0.f;
+            }
+            fold[i & 7] = lanes_fold(pr, p.lane);
+            if ((i & 7) == 0) (bco + ((int64_t)tile * 2 + (i >> 3)) * W * 64)[(uint32_t)p.lane] = tokens_fold(fold, p.lane);
         });
 #pragma unroll
         for (int s = 0; s < 4; ++s) dA[s] += tA[s];
@@ -753,11 +699,11 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const float* __rest
 
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)                  // (fewer waves have more tokens a lane: 256 registers would spill)
-scan_bwd_kernel(const Scan a, const float* __restrict__ bc0) {
+scan_bwd_kernel(const Scan a) {
     extern __shared__ __attribute__((aligned(16))) float smem[];
     const ScanPlace p(a, a.nchunk, 0);
-    if (p.cb * SC + SC <= a.Dg) scan_bwd_body<T, W, Z, true>(a, bc0, p, smem);
-    else scan_bwd_body<T, W, Z, false>(a, bc0, p, smem);
+    if (p.cb * SC + SC <= a.Dg) scan_bwd_body<T, W, Z, true>(a, p, smem);
+    else scan_bwd_body<T, W, Z, false>(a, p, smem);
 }
 
 // What the backward kernel's blocks left in shares, each sum in a fixed order: the first `bcs` blocks take dB and dC
@@ -867,7 +813,6 @@ scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const f
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-static bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
 static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 
 // How many chunks a row is cut into.  A compute unit holds six blocks of the forward kernel or two of the backward.  k of them
@@ -918,9 +863,7 @@ static void scan_shape(Scan* a, const rst_scan_desc* s, bool bwd) {
     scan_plan(a, bwd);
 }
 
-// Scratch of a call, carved from the caller's workspace (base == null: only measured).  B and C laid out for the waves are
-// kept with the states for the backward pass, where there is one.
-static int64_t scan_bc_floats(const Scan& a) { return (int64_t)a.B * a.G * a.tiles * ST * scan_waves(a.N) * 8; }
+// Scratch of a call, carved from the caller's workspace (base == null: only measured)
 static size_t scan_carve(Scan* a, char* base, bool bwd) {
     const int W = scan_waves(a->N);
     size_t off = 0;
@@ -930,30 +873,16 @@ static size_t scan_carve(Scan* a, char* base, bool bwd) {
         return p;
     };
     const int64_t chunks = (int64_t)a->B * a->nchunk;
-    if (!bwd) a->bc = take(scan_bc_floats(*a));
     if (a->nchunk > 1) {
         a->cst = take(chunks * 4 * W * a->D);
         a->cdt = take(chunks * a->D);
     }
     if (bwd) {
-        a->bcpart = take(scan_bc_floats(*a) * a->cb);
+        a->bcpart = take((int64_t)a->cb * a->B * a->G * a->tiles * 2 * W * 64);
         a->dApart = take(chunks * 4 * W * a->D);
         a->dDpart = take(chunks * 2 * a->D);
     }
     return off;
-}
-static void scan_saved(Scan* a, float* saved) {
-    a->bc = saved;
-    a->ckpt = saved + scan_bc_floats(*a);
-}
-
-template <typename T>
-static int scan_prep(const Scan& a, int W, hipStream_t st) {
-    const int64_t Lp = (int64_t)a.tiles * ST;
-    hipLaunchKernelGGL((bc_prep_kernel<T>), dim3((unsigned)cdiv(Lp, 64), a.B * a.G), dim3(256), 0, st, static_cast<const T*>(a.Bm),
-                       static_cast<const T*>(a.Cm), a.bc, a.N, W, a.L, Lp);
-    RST_LAUNCH_CHECK();
-    return RST_OK;
 }
 
 template <bool REV>
@@ -969,15 +898,14 @@ template <typename T, int W, bool Z>
 static int scan_fwd_t(const Scan& a, hipStream_t st) {
     const double n = (double)a.B * a.D * a.L;
     ProfScope prof(st, "scan_fwd", n * (7.0 * a.N + 12), sizeof(T) * n * (a.z ? 4 : 3));
-    RST_TRY(scan_prep<T>(a, W, st));
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a);
         RST_LAUNCH_CHECK();
         RST_TRY(scan_chain<false>(a, 4 * W, st));
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a, a.bc);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
@@ -989,14 +917,14 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a, a.bc);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a);
         RST_LAUNCH_CHECK();
         RST_TRY(scan_chain<true>(a, 4 * W, st));
     }
     const size_t lds = (size_t)(3 + (Z ? 3 : 2) * W) * ST * SROW * sizeof(float);
     KernelSetup ks;
     RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W, Z>), 64 * W, lds, &ks));
-    hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a, a.bc);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a);
     RST_LAUNCH_CHECK();
     const int64_t bcs = cdiv(a.L, 64) * a.B * a.G, all = bcs + cdiv(a.D, 16) * (a.N + 2);
     RST_REQUIRE(all < (1ll << 31), "scan: grid out of range");
@@ -1035,7 +963,7 @@ size_t rst_scan_saved_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_saved_bytes", s) != RST_OK) return 0;
     Scan a{};
     scan_shape(&a, s, true);
-    return ((size_t)scan_bc_floats(a) + (size_t)a.B * a.tiles * 4 * scan_waves(a.N) * a.D) * sizeof(float);
+    return (size_t)a.B * a.tiles * 4 * scan_waves(a.N) * a.D * sizeof(float);
 }
 size_t rst_scan_bwd_workspace_bytes(const rst_scan_desc* s) {
     if (scan_check("scan_bwd_workspace_bytes", s) != RST_OK) return 0;
@@ -1051,13 +979,12 @@ int rst_scan_fwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     Scan a{};
     scan_shape(&a, s, false);
     const size_t need = scan_carve(&a, nullptr, false);
-    if (workspace == nullptr || workspace_bytes < need)
+    if (need && (workspace == nullptr || workspace_bytes < need))
         return fail(RST_ERR_WORKSPACE, "scan_fwd: workspace too small (%zu < %zu)", workspace_bytes, need);
-    RST_REQUIRE(aligned256(workspace) && aligned256(saved), "scan_fwd: workspace or saved not aligned to 256 bytes");
+    RST_REQUIRE(aligned16(workspace), "scan_fwd: workspace not aligned to 16 bytes");
     scan_carve(&a, static_cast<char*>(workspace), false);
     a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
-    a.h0 = state_in; a.y = y; a.last = state_out;
-    if (saved) scan_saved(&a, saved);
+    a.h0 = state_in; a.y = y; a.last = state_out; a.ckpt = saved;
     const int W = scan_waves(a.N);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define FWD(T, W_) (a.z ? scan_fwd_t<T, W_, true>(a, st) : scan_fwd_t<T, W_, false>(a, st))
@@ -1075,11 +1002,10 @@ int rst_scan_bwd(const rst_scan_desc* s, const rst_scan_inputs* in, const float*
     const size_t need = scan_carve(&a, nullptr, true);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(RST_ERR_WORKSPACE, "scan_bwd: workspace too small (%zu < %zu)", workspace_bytes, need);
-    RST_REQUIRE(aligned256(workspace) && aligned256(saved), "scan_bwd: workspace or saved not aligned to 256 bytes");
+    RST_REQUIRE(aligned16(workspace), "scan_bwd: workspace not aligned to 16 bytes");
     scan_carve(&a, static_cast<char*>(workspace), true);
     a.x = in->x; a.delta = in->delta; a.A = in->A; a.Bm = in->B; a.Cm = in->C; a.Dskip = in->D; a.z = in->z; a.dbias = in->delta_bias;
-    scan_saved(&a, const_cast<float*>(saved));
-    a.dy = dy; a.dlast = dstate_out;
+    a.ckpt = const_cast<float*>(saved); a.dy = dy; a.dlast = dstate_out;
     a.dx = out->x; a.ddelta = out->delta; a.dB = out->B; a.dC = out->C; a.dz = out->z; a.dh0 = dstate_in;
     const int W = scan_waves(a.N);
     hipStream_t st = static_cast<hipStream_t>(stream);

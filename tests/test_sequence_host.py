@@ -190,13 +190,16 @@ def test_c_entry_points_refuse():
 
     def desc(B=1, D=4, G=1, N=8, L=10, dtype=0):
         return ctypes.byref(_lib.ScanDesc(B, D, G, N, L, dtype, 1))
-    for kw in (dict(B=0), dict(D=0), dict(L=0), dict(N=0), dict(N=33), dict(G=3), dict(G=0), dict(dtype=7), dict(B=70000), dict(L=(1 << 24) + 1)):
-        assert lib.rst_scan_workspace_bytes(desc(**kw)) == 0, kw
-        assert lib.rst_scan_saved_bytes(desc(**kw)) == 0 and lib.rst_scan_bwd_workspace_bytes(desc(**kw)) == 0
     ins = _lib.ScanInputs(p, p, p, p, p, None, None, None)
-    need = lib.rst_scan_workspace_bytes(desc())
-    assert lib.rst_scan_fwd(desc(), ctypes.byref(ins), None, p, None, None, p, need - 1, None) == 3
-    assert lib.rst_scan_fwd(desc(), ctypes.byref(ins), None, p, None, None, p + 4, need, None) == 1 and "aligned" in err()
+    for kw in (dict(B=0), dict(D=0), dict(L=0), dict(N=0), dict(N=33), dict(G=3), dict(G=0), dict(dtype=7), dict(B=70000), dict(L=(1 << 24) + 1)):
+        assert lib.rst_scan_saved_bytes(desc(**kw)) == 0 and lib.rst_scan_bwd_workspace_bytes(desc(**kw)) == 0
+        assert lib.rst_scan_fwd(desc(**kw), ctypes.byref(ins), None, p, None, None, p, 1 << 40, None) == 1, kw
+    assert lib.rst_scan_workspace_bytes(desc()) == 0                      # one chunk: no scratch
+    need = lib.rst_scan_workspace_bytes(desc(L=5000))
+    assert need > 0
+    assert lib.rst_scan_fwd(desc(L=5000), ctypes.byref(ins), None, p, None, None, p, need - 1, None) == 3
+    assert lib.rst_scan_fwd(desc(L=5000), ctypes.byref(ins), None, p, None, None, None, need, None) == 3
+    assert lib.rst_scan_fwd(desc(L=5000), ctypes.byref(ins), None, p, None, None, p + 4, need, None) == 1 and "aligned" in err()
     assert lib.rst_scan_fwd(desc(), ctypes.byref(_lib.ScanInputs(p, p, p, p, None, None, None, None)), None, p, None, None, p, need, None) == 1
     outs = _lib.ScanGrads(p, p, p, p, p, None, None, None)
     need = lib.rst_scan_bwd_workspace_bytes(desc())
