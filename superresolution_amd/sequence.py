@@ -32,22 +32,27 @@ MAX_TOKENS = 1 << 24     # of a row of the scan
 # ----------------------------------------------------------------------------
 # plumbing
 # ----------------------------------------------------------------------------
-def _act(t: torch.Tensor, op: str, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """An activation: fp32 or bf16 on a ROCm device, of `like`'s type and device."""
-    if not t.is_cuda:
-        raise RuntimeError(f"{op} {what}: tensor is on {t.device}; this operator only runs on a ROCm GPU "
-                           "(there is no CPU fallback)")
-    if t.dtype not in _DTYPES:
-        raise RuntimeError(f"{op} {what}: dtype {t.dtype} not supported (fp32 or bf16)")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise RuntimeError(f"{op} {what}: {t.dtype} on {t.device}, but x is {like.dtype} on {like.device}")
+def _act(t: torch.Tensor, op: str, what: str, like: Optional[torch.Tensor] = None, want: Optional[tuple] = None) -> torch.Tensor:
+    """An activation: fp32 or bf16 on a ROCm device, of `like`'s type and device and of the shape `want`."""
+    if want is not None and t.shape != want:
+        _wrong_shape(t, op, what, want)
+    if like is None or t.dtype is not like.dtype or t.device != like.device:     # `like` is one that was looked at
+        if not t.is_cuda:
+            raise RuntimeError(f"{op} {what}: tensor is on {t.device}; this operator only runs on a ROCm GPU "
+                               "(there is no CPU fallback)")
+        if t.dtype not in _DTYPES:
+            raise RuntimeError(f"{op} {what}: dtype {t.dtype} not supported (fp32 or bf16)")
+        if like is not None:
+            raise RuntimeError(f"{op} {what}: {t.dtype} on {t.device}, but x is {like.dtype} on {like.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _par(t: Optional[torch.Tensor], op: str, what: str, like: torch.Tensor) -> Optional[torch.Tensor]:
-    """A parameter or a state of the scan: fp32 on `like`'s device, or None."""
+def _par(t: Optional[torch.Tensor], op: str, what: str, like: torch.Tensor, want: Optional[tuple] = None) -> Optional[torch.Tensor]:
+    """A parameter or a state of the scan: fp32 on `like`'s device, of the shape `want`; or None."""
     if t is None:
         return None
+    if want is not None and t.shape != want:
+        _wrong_shape(t, op, what, want)
     if t.device != like.device:
         raise RuntimeError(f"{op} {what}: tensor is on {t.device}, but x is on {like.device}")
     if t.dtype != torch.float32:
@@ -55,9 +60,8 @@ def _par(t: Optional[torch.Tensor], op: str, what: str, like: torch.Tensor) -> O
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _shape(t: Optional[torch.Tensor], op: str, what: str, want: tuple) -> None:
-    if t is not None and t.shape != want:
-        raise RuntimeError(f"{op} {what}: shape {tuple(t.shape)}, expected {want}")
+def _wrong_shape(t: torch.Tensor, op: str, what: str, want: tuple) -> None:
+    raise RuntimeError(f"{op} {what}: shape {tuple(t.shape)}, expected {tuple(want)}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -103,14 +107,15 @@ def _wants_grad(*tensors) -> bool:
 def _next_state(state: torch.Tensor, state_out: Optional[torch.Tensor], name: str) -> torch.Tensor:
     """Where an update writes the next state: `state` itself, or a tensor of its own."""
     out = state if state_out is None else state_out
-    if out.shape != state.shape or out.dtype != state.dtype or out.device != state.device:
-        raise RuntimeError(f"{name}: state_out is {out.dtype} {tuple(out.shape)} on {out.device}, "
-                           f"state {state.dtype} {tuple(state.shape)} on {state.device}")
     if not out.is_contiguous():
         raise RuntimeError(f"{name}: the state is written in place and has to be contiguous (strides {out.stride()})")
-    size = out.numel() * out.element_size()
-    if out.data_ptr() != state.data_ptr() and abs(out.data_ptr() - state.data_ptr()) < size:
-        raise RuntimeError(f"{name}: state_out overlaps state")
+    if state_out is not None:
+        if out.shape != state.shape or out.dtype != state.dtype or out.device != state.device:
+            raise RuntimeError(f"{name}: state_out is {out.dtype} {tuple(out.shape)} on {out.device}, "
+                               f"state {state.dtype} {tuple(state.shape)} on {state.device}")
+        gap = abs(out.data_ptr() - state.data_ptr())
+        if gap and gap < out.numel() * out.element_size():
+            raise RuntimeError(f"{name}: state_out overlaps state")
     return out
 
 
@@ -158,10 +163,8 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
         raise RuntimeError(f"layernorm: x {tuple(x.shape)} (the last dimension: 1 to {MAX_NORM_WIDTH})")
     if not eps >= 0:
         raise RuntimeError(f"layernorm: eps={eps} is negative or no number")
-    x = _act(x, "layernorm", "x")
-    _shape(weight, "layernorm", "weight", (x.shape[-1],))
-    _shape(bias, "layernorm", "bias", (x.shape[-1],))
-    weight, bias = _par(weight, "layernorm", "weight", x), _par(bias, "layernorm", "bias", x)
+    x, want = _act(x, "layernorm", "x"), x.shape[-1:]
+    weight, bias = _par(weight, "layernorm", "weight", x, want), _par(bias, "layernorm", "bias", x, want)
     if _wants_grad(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps))
@@ -224,8 +227,7 @@ def _conv_args(name, x, weight, bias, activation):
     D = x.shape[1]
     if weight.dim() != 2 or weight.shape[0] != D or not 2 <= weight.shape[1] <= 4:
         raise RuntimeError(f"{name}: weight {tuple(weight.shape)} does not fit {D} channels and 2 to 4 taps")
-    _shape(bias, name, "bias", (D,))
-    return x, _par(weight, name, "weight", x), _par(bias, name, "bias", x)
+    return x, _par(weight, name, "weight", x), _par(bias, name, "bias", x, (D,))
 
 
 def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -239,8 +241,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise RuntimeError(f"causal_conv1d: x {tuple(x.shape)} (batch, channel, token)")
     x, weight, bias = _conv_args("causal_conv1d", x, weight, bias, activation)
     if initial_state is not None:
-        _shape(initial_state, "causal_conv1d", "initial_state", (x.shape[0], x.shape[1], weight.shape[1] - 1))
-        initial_state = _act(initial_state, "causal_conv1d", "initial_state", x)
+        initial_state = _act(initial_state, "causal_conv1d", "initial_state", x, (x.shape[0], x.shape[1], weight.shape[1] - 1))
     if _wants_grad(x, weight, bias, initial_state):
         return _CausalConvFn.apply(x, weight, bias, initial_state, activation == "silu", bool(return_final_state))
     y, end = _conv_forward(x, weight, bias, initial_state, activation == "silu", return_final_state)
@@ -257,8 +258,8 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
         raise RuntimeError("causal_conv1d_update is inference only: call it under torch.no_grad()")
     x, weight, bias = _conv_args("causal_conv1d_update", x, weight, bias, activation)
     B, D, W = x.shape[0], x.shape[1], weight.shape[1]
-    _shape(state, "causal_conv1d_update", "state", (B, D, W - 1))
-    state, out = _act(state, "causal_conv1d_update", "state", x), _next_state(state, state_out, "causal_conv1d_update")
+    out = _next_state(state, state_out, "causal_conv1d_update")
+    state = _act(state, "causal_conv1d_update", "state", x, (B, D, W - 1))
     y = torch.empty_like(x)
     if x.numel():
         _call("rst_causal_conv1d_update", x, x.data_ptr(), _DTYPES[x.dtype], state.data_ptr(), out.data_ptr(), weight.data_ptr(),
@@ -329,24 +330,21 @@ class _ScanFn(torch.autograd.Function):
 
 def _scan_args(name, x, delta, A, B, C, D, z, delta_bias):
     x = _act(x, name, "x")
-    batch, chan, tail = x.shape[0], x.shape[1], tuple(x.shape[2:])
+    size = x.shape
+    chan, dims = size[1], len(size)
     if A.dim() != 2 or A.shape[0] != chan or not 1 <= A.shape[1] <= MAX_STATES:
         raise RuntimeError(f"{name}: A {tuple(A.shape)} does not fit {chan} channels and 1 to {MAX_STATES} states")
-    if B.dim() == x.dim():                                   # one group: (B, N, L) for (B, 1, N, L)
+    if B.dim() == dims:                                      # one group: (B, N, L) for (B, 1, N, L)
         B = B.unsqueeze(1)
-    if C.dim() == x.dim():
+    if C.dim() == dims:
         C = C.unsqueeze(1)
-    groups = B.shape[1] if B.dim() == x.dim() + 1 else 0
+    groups = B.shape[1] if B.dim() == dims + 1 else 0
     if groups < 1 or chan % groups:
         raise RuntimeError(f"{name}: B {tuple(B.shape)}: {chan} channels are not divisible into its groups")
-    _shape(B, name, "B", (batch, groups, A.shape[1]) + tail)
-    _shape(C, name, "C", (batch, groups, A.shape[1]) + tail)
-    _shape(delta, name, "delta", x.shape)
-    _shape(z, name, "z", x.shape)
-    _shape(D, name, "D", (chan,))
-    _shape(delta_bias, name, "delta_bias", (chan,))
-    return (x, _act(delta, name, "delta", x), _par(A, name, "A", x), _act(B, name, "B", x), _act(C, name, "C", x),
-            _par(D, name, "D", x), None if z is None else _act(z, name, "z", x), _par(delta_bias, name, "delta_bias", x))
+    want = (size[0], groups, A.shape[1]) + size[2:]
+    return (x, _act(delta, name, "delta", x, size), _par(A, name, "A", x), _act(B, name, "B", x, want),
+            _act(C, name, "C", x, want), _par(D, name, "D", x, (chan,)), None if z is None else _act(z, name, "z", x, size),
+            _par(delta_bias, name, "delta_bias", x, (chan,)))
 
 
 def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
@@ -372,8 +370,7 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
         raise RuntimeError(f"selective_scan: {x.shape[2]} tokens (at most {MAX_TOKENS}: carry the state on in pieces)")
     args = _scan_args("selective_scan", x, delta, A, B, C, D, z, delta_bias)
     x, A = args[0], args[2]
-    _shape(initial_state, "selective_scan", "initial_state", (x.shape[0], x.shape[1], A.shape[1]))
-    h0 = _par(initial_state, "selective_scan", "initial_state", x)
+    h0 = _par(initial_state, "selective_scan", "initial_state", x, (x.shape[0], x.shape[1], A.shape[1]))
     if _wants_grad(*args, h0):
         return _ScanFn.apply(*args, h0, bool(delta_softplus), bool(return_last_state))
     y, last, _ = _scan_forward(*args, h0, delta_softplus, return_last_state, False)
@@ -391,8 +388,8 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     if _wants_grad(state, x, delta, A, B, C, D, z, delta_bias):
         raise RuntimeError("selective_scan_update is inference only: call it under torch.no_grad()")
     x, delta, A, B, C, D, z, delta_bias = _scan_args("selective_scan_update", x, delta, A, B, C, D, z, delta_bias)
-    _shape(state, "selective_scan_update", "state", (x.shape[0], x.shape[1], A.shape[1]))
-    state, out = _par(state, "selective_scan_update", "state", x), _next_state(state, state_out, "selective_scan_update")
+    out = _next_state(state, state_out, "selective_scan_update")
+    state = _par(state, "selective_scan_update", "state", x, x.shape + A.shape[1:])
     y = torch.empty_like(x)
     if x.numel():
         desc, ins = _scan_desc(x, A, B, delta_softplus), _scan_inputs(x, delta, A, B, C, D, z, delta_bias)
