@@ -209,6 +209,7 @@ __device__ __forceinline__ float gate_of(const Quad<T>& z, int i) {
 }
 
 // ---- what a chunk adds to the state behind it (REV: to the state's gradient before it), and the sum of its dt -------
+// 8 x 384 x 16384 bf16 of 16 states: 167 us, REV with a gate 186 (4.8 and 4.3 T state updates a second).
 template <typename T, int W, bool Z, bool REV>
 __global__ void __launch_bounds__(64 * W, 8)                               // (at most 256 registers: else the matrix results go to AGPRs and back)
 scan_chunk_kernel(const Scan a) {
@@ -297,7 +298,7 @@ scan_chunk_kernel(const Scan a) {
 // ---- the chunks' own states, one behind the other: cst[c] becomes the state that chunk c starts from (REV: the
 // state's gradient behind it).  A block has 64 channels and one state; its waves take a run of chunks each, side by side,
 // chain the runs through LDS and walk their run again: four waves with up to 8 chunks each, or 16 with 16; what a run of that
-// length reads stays in registers for the second walk.  (Chained in front of every chunk by the scan's own blocks, the
+// length reads stays in registers for the second walk: 5.7 us for 32 chunks of 8 x 384 channels, 8.4 for 256 of 192.  (Chained in front of every chunk by the scan's own blocks, the
 // states are read as often as there are chunks: 503 MB from the caches for 256 chunks of 192 channels, 45 us instead of 20.)
 // A state of zero stays zero over a chunk whose decay overflows (growing states, A > 0): 0 times infinity is no number.
 __device__ __forceinline__ float over_chunk(float h, float sum, float A, float own) {
@@ -362,6 +363,8 @@ __device__ __forceinline__ float start_state(const Scan& a, const ScanPlace& p, 
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
+// 8 x 384 x 16384 bf16 of 16 states, gated, the states before every tile kept: 261 us (3.1 T state updates a second; 604 MB, 2.3
+// TB/s).  80 registers and 25.5 KiB: six blocks a compute unit.
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, 6)
 scan_fwd_kernel(const Scan a) {
@@ -697,6 +700,8 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const ScanPlace& p,
     }
 }
 
+// 8 x 384 x 16384 bf16 of 16 states, gated: 793 us (1.0 T state updates a second): the 256 registers that hold the tile's states and
+// decays leave two waves a SIMD, which keep the vector pipe busy 75 % of the time (forward: six, 82 %).
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)                  // (fewer waves have more tokens a lane: 256 registers would spill)
 scan_bwd_kernel(const Scan a) {
@@ -754,7 +759,8 @@ scan_reduce_kernel(const Scan a, int W, int bcs, float* __restrict__ dA, float* 
 }
 
 // ---- one token -----------------------------------------------------------------------------------------------------
-// NL lanes share a channel, four states each.  Bound by the state's 8 N bytes per channel.  state_out may be the state.
+// NL lanes share a channel, four states each.  Bound by the state's 8 N bytes per channel (256 x 768 of 16 states: 9.5 us, 2.7
+// TB/s; 1 x 384: 3.5 us, a launch).  state_out may be the state.
 template <typename T, int NL>
 __global__ void __launch_bounds__(256)
 scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const float* __restrict__ A, const T* __restrict__ Bm,
@@ -820,8 +826,9 @@ static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
 // clock and compute unit with one, two, four and eight waves, so one alone takes 2.4 shares (backward 1.9) and k take about
 // k + 1/2 (backward k).  Chunks cost the pass over their own states, 0.6 of the forward kernel's time and 0.2 of the
 // backward's, a block about half a tile beside its tiles, and the chain about three.  The number that costs least is
-// taken, chunks of at least two tiles.  Measured, 8 x 384 x 16384 bf16: forward 612, 529, 500, 468, 480 us with 10, 16, 21, 32, 48
-// chunks, backward 1804, 1227, 1125, 1095 with 5, 10, 21, 32; one 16384-token prompt of 192 channels 60 us with 512, 52 with 256.
+// taken, chunks of at least two tiles.  Measured, 8 x 384 x 16384 bf16: forward 784, 546, 463, 449, 440, 454 us with 5, 10, 16,
+// 21, 32, 48 chunks, backward 1497, 1068, 1065, 1020, 1020, 1047; one 16384-token prompt of 192 channels 70, 61, 53, 46, 45, 46
+// us with 64, 85, 128, 171, 256, 512.
 static void scan_plan(Scan* a, bool bwd) {
     a->Dg = a->D / a->G;
     a->cb = (int)cdiv(a->Dg, SC);
