@@ -607,3 +607,36 @@ def test_offsets_beyond_32_bits():
     assert float((y[-1, :, -200:].float() - want[0].float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
     assert float((last[-1] - end[0]).abs().max()) <= 64 * 2.0 ** -24 * float(end.abs().max())
     assert not y[-1, :, :-200].any() and not y[0].any()
+
+
+def test_longest_row_with_the_most_states():
+    """2^24 tokens and 32 states: the furthest offsets into B, C, the kept states and the shares of dB and dC.  Nothing enters the
+    state or its gradient before the last 200 tokens, so those alone give the same.  Every term is positive there, so that two
+    results that are each off by n 2^-24 of their terms' sum differ by no more than 2 n 2^-24 of themselves."""
+    L, D, N, K = sequence.MAX_TOKENS, 2, 32, 200
+    gen = torch.Generator(device="cuda").manual_seed(5)
+
+    def rand(*shape):
+        return torch.rand(*shape, generator=gen, device="cuda") + 0.5
+
+    def late(t):
+        t[..., :-K] = 0
+        return t
+    x, dy = late(rand(1, D, L)), late(rand(1, D, L))
+    delta = torch.full((1, D, L), 0.3, device="cuda")
+    A = -torch.linspace(0.2, 2.0, D * N, device="cuda").view(D, N)
+    B, C = rand(1, 1, N, L), rand(1, 1, N, L)
+
+    def grads(*ins):
+        ins = [t.detach().contiguous().requires_grad_(True) for t in ins]
+        y, last = sequence.selective_scan(ins[0], ins[1], A, ins[2], ins[3], return_last_state=True)
+        gr = torch.autograd.grad(y, (ins[0], ins[2], ins[3]), dy[..., -y.shape[2]:].contiguous())
+        return (y.detach(), last.detach()) + gr
+    whole = grads(x, delta, B, C)
+    end = grads(x[..., -K:], delta[..., -K:], B[..., -K:], C[..., -K:])
+    n = 8 * K + N + D + 1 + 80
+    for name, w, e in zip(("y", "last", "dx", "dB", "dC"), whole, end):
+        w = w[..., -K:] if name != "last" else w
+        assert e.min() > 0, name
+        assert float(((w - e).abs() / e).max()) <= 2 * n * 2.0 ** -24, name
+    assert not whole[0][..., :-K].any() and not whole[3][..., :-K].any() and not whole[4][..., :-K].any()
