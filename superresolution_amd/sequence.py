@@ -10,8 +10,8 @@ eager fallback.
 
 Inputs of other strides are copied to contiguous ones, as everywhere in this package.  Work goes to the current stream
 of the inputs' device, whichever device is current; scratch comes from torch's allocator call by call, so calls on two
-streams and captured graphs share none.  Gradients are first-order only.  A captured backward pass needs what torch needs of any:
-leaves without a live eager graph (capture a function that calls ``torch.autograd.grad``).
+streams and captured graphs share none.  Gradients are first-order and reverse-mode only; others are refused.  A
+captured backward pass needs what torch needs of any: leaves without a live eager graph (capture a function that calls ``torch.autograd.grad``).
 """
 from __future__ import annotations
 
@@ -19,6 +19,7 @@ import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ScanDesc, ScanGrads, ScanInputs, check
@@ -96,12 +97,23 @@ def _scratch(nbytes: int, t: torch.Tensor) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
 
 
-def _wants_grad(*tensors) -> bool:
+def _wants_grad(name: str, *tensors) -> bool:
+    """Whether a call has to be differentiable.  A dual tensor of forward-mode differentiation has requires_grad == False:
+    it is refused, since the way without gradients would drop its tangent."""
+    if forward_ad._current_level >= 0:           # inside dual_level(): -1 without one
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _inference_only(name: str, *tensors) -> None:
+    if _wants_grad(name, *tensors):
+        raise RuntimeError(f"{name} is inference only: call it under torch.no_grad()")
 
 
 def _next_state(state: torch.Tensor, state_out: Optional[torch.Tensor], name: str) -> torch.Tensor:
@@ -165,7 +177,7 @@ def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
         raise RuntimeError(f"layernorm: eps={eps} is negative or no number")
     x, want = _act(x, "layernorm", "x"), x.shape[-1:]
     weight, bias = _par(weight, "layernorm", "weight", x, want), _par(bias, "layernorm", "bias", x, want)
-    if _wants_grad(x, weight, bias):
+    if _wants_grad("layernorm", x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps))
 
@@ -242,7 +254,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     x, weight, bias = _conv_args("causal_conv1d", x, weight, bias, activation)
     if initial_state is not None:
         initial_state = _act(initial_state, "causal_conv1d", "initial_state", x, (x.shape[0], x.shape[1], weight.shape[1] - 1))
-    if _wants_grad(x, weight, bias, initial_state):
+    if _wants_grad("causal_conv1d", x, weight, bias, initial_state):
         return _CausalConvFn.apply(x, weight, bias, initial_state, activation == "silu", bool(return_final_state))
     y, end = _conv_forward(x, weight, bias, initial_state, activation == "silu", return_final_state)
     return (y, end) if return_final_state else y
@@ -254,8 +266,7 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     `state_out` and stays.  Inference only."""
     if x.dim() != 2:
         raise RuntimeError(f"causal_conv1d_update: x {tuple(x.shape)} (batch, channel)")
-    if _wants_grad(x, state, weight, bias):
-        raise RuntimeError("causal_conv1d_update is inference only: call it under torch.no_grad()")
+    _inference_only("causal_conv1d_update", x, state, weight, bias)
     x, weight, bias = _conv_args("causal_conv1d_update", x, weight, bias, activation)
     B, D, W = x.shape[0], x.shape[1], weight.shape[1]
     out = _next_state(state, state_out, "causal_conv1d_update")
@@ -371,7 +382,7 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     args = _scan_args("selective_scan", x, delta, A, B, C, D, z, delta_bias)
     x, A = args[0], args[2]
     h0 = _par(initial_state, "selective_scan", "initial_state", x, (x.shape[0], x.shape[1], A.shape[1]))
-    if _wants_grad(*args, h0):
+    if _wants_grad("selective_scan", *args, h0):
         return _ScanFn.apply(*args, h0, bool(delta_softplus), bool(return_last_state))
     y, last, _ = _scan_forward(*args, h0, delta_softplus, return_last_state, False)
     return (y, last) if return_last_state else y
@@ -385,8 +396,7 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     state).  `state` (batch, channel, state), fp32, moves on in place, or into `state_out` and stays.  Inference only."""
     if x.dim() != 2:
         raise RuntimeError(f"selective_scan_update: x {tuple(x.shape)} (batch, channel)")
-    if _wants_grad(state, x, delta, A, B, C, D, z, delta_bias):
-        raise RuntimeError("selective_scan_update is inference only: call it under torch.no_grad()")
+    _inference_only("selective_scan_update", state, x, delta, A, B, C, D, z, delta_bias)
     x, delta, A, B, C, D, z, delta_bias = _scan_args("selective_scan_update", x, delta, A, B, C, D, z, delta_bias)
     out = _next_state(state, state_out, "selective_scan_update")
     state = _par(state, "selective_scan_update", "state", x, x.shape + A.shape[1:])

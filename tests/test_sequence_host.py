@@ -214,3 +214,36 @@ def test_the_longest_row(fake):
     with pytest.raises(RuntimeError, match="at most 16777216"):
         sequence.selective_scan(fake(1, 2, (1 << 24) + 1), fake(1, 2, (1 << 24) + 1), fake(2, 1), fake(1, 1, 1, (1 << 24) + 1),
                                 fake(1, 1, 1, (1 << 24) + 1))
+
+
+# ---- forward-mode derivatives: there are none, and none is dropped ---------------------------------------------------
+def _dual_calls(make):
+    """Each entry point with every one of its tensors in turn, as (name, call of that tensor's dual)."""
+    x, w = make(2, 6, 10), make(6, 4)
+    x1, w1, s1 = make(2, 6), make(6, 4), make(2, 6, 3)
+    A, B, B1, v, h = make(6, 8), make(2, 1, 8, 10), make(2, 1, 8), make(6), make(2, 6, 8)
+    sq = sequence
+    table = [(lambda x, w, b: sq.layernorm(x, w, b), [make(2, 8), make(8), make(8)]),
+             (lambda x, w, b, h: sq.causal_conv1d(x, w, b, initial_state=h, activation="silu"), [x, w, v, s1]),
+             (lambda x, s, w, b: sq.causal_conv1d_update(x, s, w, b), [x1, s1, w1, v]),
+             (lambda x, d, A, B, C, D, z, b, h: sq.selective_scan(x, d, A, B, C, D, z=z, delta_bias=b, initial_state=h),
+              [x, x, A, B, B, v, x, v, h]),
+             (lambda s, x, d, A, B, C, D, z, b: sq.selective_scan_update(s, x, d, A, B, C, D, z=z, delta_bias=b),
+              [h, x1, x1, A, B1, B1, v, x1, v])]
+    for call, tensors in table:
+        for i, t in enumerate(tensors):
+            yield lambda dual, call=call, tensors=tensors, i=i: call(*tensors[:i], dual, *tensors[i + 1:]), t
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(fake, monkeypatch, grad):
+    """A dual tensor has requires_grad == False: it must not take the way without gradients, whose result has no tangent."""
+    monkeypatch.setattr(sequence, "_call", lambda name, *args: pytest.fail(f"{name} was launched"))
+    fw = torch.autograd.forward_ad
+    n = 0
+    for call, t in _dual_calls(fake):
+        with fw.dual_level(), torch.set_grad_enabled(grad):
+            with pytest.raises(NotImplementedError):
+                call(fw.make_dual(t, torch.ones_like(t)))
+        n += 1
+    assert n == 29
