@@ -266,7 +266,7 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     `state_out` and stays.  Inference only."""
     if x.dim() != 2:
         raise RuntimeError(f"causal_conv1d_update: x {tuple(x.shape)} (batch, channel)")
-    _inference_only("causal_conv1d_update", x, state, weight, bias)
+    _inference_only("causal_conv1d_update", x, state, weight, bias, state_out)
     x, weight, bias = _conv_args("causal_conv1d_update", x, weight, bias, activation)
     B, D, W = x.shape[0], x.shape[1], weight.shape[1]
     out = _next_state(state, state_out, "causal_conv1d_update")
@@ -396,7 +396,7 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     state).  `state` (batch, channel, state), fp32, moves on in place, or into `state_out` and stays.  Inference only."""
     if x.dim() != 2:
         raise RuntimeError(f"selective_scan_update: x {tuple(x.shape)} (batch, channel)")
-    _inference_only("selective_scan_update", state, x, delta, A, B, C, D, z, delta_bias)
+    _inference_only("selective_scan_update", state, x, delta, A, B, C, D, z, delta_bias, state_out)
     x, delta, A, B, C, D, z, delta_bias = _scan_args("selective_scan_update", x, delta, A, B, C, D, z, delta_bias)
     out = _next_state(state, state_out, "selective_scan_update")
     state = _par(state, "selective_scan_update", "state", x, x.shape + A.shape[1:])

@@ -225,11 +225,11 @@ def _dual_calls(make):
     sq = sequence
     table = [(lambda x, w, b: sq.layernorm(x, w, b), [make(2, 8), make(8), make(8)]),
              (lambda x, w, b, h: sq.causal_conv1d(x, w, b, initial_state=h, activation="silu"), [x, w, v, s1]),
-             (lambda x, s, w, b: sq.causal_conv1d_update(x, s, w, b), [x1, s1, w1, v]),
+             (lambda x, s, w, b, o: sq.causal_conv1d_update(x, s, w, b, state_out=o), [x1, s1, w1, v, make(2, 6, 3)]),
              (lambda x, d, A, B, C, D, z, b, h: sq.selective_scan(x, d, A, B, C, D, z=z, delta_bias=b, initial_state=h),
               [x, x, A, B, B, v, x, v, h]),
-             (lambda s, x, d, A, B, C, D, z, b: sq.selective_scan_update(s, x, d, A, B, C, D, z=z, delta_bias=b),
-              [h, x1, x1, A, B1, B1, v, x1, v])]
+             (lambda s, x, d, A, B, C, D, z, b, o: sq.selective_scan_update(s, x, d, A, B, C, D, z=z, delta_bias=b, state_out=o),
+              [h, x1, x1, A, B1, B1, v, x1, v, make(2, 6, 8)])]
     for call, tensors in table:
         for i, t in enumerate(tensors):
             yield lambda dual, call=call, tensors=tensors, i=i: call(*tensors[:i], dual, *tensors[i + 1:]), t
@@ -246,4 +246,13 @@ def test_forward_mode_tangents_are_refused(fake, monkeypatch, grad):
             with pytest.raises(NotImplementedError):
                 call(fw.make_dual(t, torch.ones_like(t)))
         n += 1
-    assert n == 29
+    assert n == 31
+
+
+def test_update_does_not_write_into_a_leaf(fake):
+    """`state_out` with a gradient of its own: torch refuses an in-place write to such a tensor, and so does an update."""
+    with pytest.raises(RuntimeError, match="inference only"):
+        sequence.causal_conv1d_update(fake(2, 6), fake(2, 6, 3), fake(6, 4), state_out=fake(2, 6, 3).requires_grad_(True))
+    with pytest.raises(RuntimeError, match="inference only"):
+        sequence.selective_scan_update(fake(2, 6, 8), fake(2, 6), fake(2, 6), fake(6, 8), fake(2, 1, 8), fake(2, 1, 8),
+                                       state_out=fake(2, 6, 8).requires_grad_(True))
