@@ -111,9 +111,9 @@ def _wants_grad(name: str, *tensors) -> bool:
     return False
 
 
-def _inference_only(name: str, *tensors) -> None:
-    if _wants_grad(name, *tensors):
-        raise RuntimeError(f"{name} is inference only: call it under torch.no_grad()")
+# tells autograd that a tensor was written to, so that a graph which saved its old values refuses them (torch.autograd.graph's
+# increment_version without its argument checks, which take twice as long)
+_increment_version = torch._C._increment_version
 
 
 def _next_state(state: torch.Tensor, state_out: Optional[torch.Tensor], name: str) -> torch.Tensor:
@@ -266,7 +266,8 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     `state_out` and stays.  Inference only."""
     if x.dim() != 2:
         raise RuntimeError(f"causal_conv1d_update: x {tuple(x.shape)} (batch, channel)")
-    _inference_only("causal_conv1d_update", x, state, weight, bias, state_out)
+    if _wants_grad("causal_conv1d_update", x, state, weight, bias, state_out):
+        raise RuntimeError("causal_conv1d_update is inference only: call it under torch.no_grad()")
     x, weight, bias = _conv_args("causal_conv1d_update", x, weight, bias, activation)
     B, D, W = x.shape[0], x.shape[1], weight.shape[1]
     out = _next_state(state, state_out, "causal_conv1d_update")
@@ -275,6 +276,7 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     if x.numel():
         _call("rst_causal_conv1d_update", x, x.data_ptr(), _DTYPES[x.dtype], state.data_ptr(), out.data_ptr(), weight.data_ptr(),
               _ptr(bias), y.data_ptr(), B, D, W, int(activation == "silu"))
+        _increment_version((out,))
     return y
 
 
@@ -396,7 +398,8 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     state).  `state` (batch, channel, state), fp32, moves on in place, or into `state_out` and stays.  Inference only."""
     if x.dim() != 2:
         raise RuntimeError(f"selective_scan_update: x {tuple(x.shape)} (batch, channel)")
-    _inference_only("selective_scan_update", state, x, delta, A, B, C, D, z, delta_bias, state_out)
+    if _wants_grad("selective_scan_update", state, x, delta, A, B, C, D, z, delta_bias, state_out):
+        raise RuntimeError("selective_scan_update is inference only: call it under torch.no_grad()")
     x, delta, A, B, C, D, z, delta_bias = _scan_args("selective_scan_update", x, delta, A, B, C, D, z, delta_bias)
     out = _next_state(state, state_out, "selective_scan_update")
     state = _par(state, "selective_scan_update", "state", x, x.shape + A.shape[1:])
@@ -404,4 +407,5 @@ def selective_scan_update(state: torch.Tensor, x: torch.Tensor, delta: torch.Ten
     if x.numel():
         desc, ins = _scan_desc(x, A, B, delta_softplus), _scan_inputs(x, delta, A, B, C, D, z, delta_bias)
         _call("rst_scan_update", x, ctypes.byref(desc), ctypes.byref(ins), state.data_ptr(), out.data_ptr(), y.data_ptr())
+        _increment_version((out,))
     return y

@@ -640,3 +640,34 @@ def test_longest_row_with_the_most_states():
         assert e.min() > 0, name
         assert float(((w - e).abs() / e).max()) <= 2 * n * 2.0 ** -24, name
     assert not whole[0][..., :-K].any() and not whole[3][..., :-K].any() and not whole[4][..., :-K].any()
+
+
+def test_a_saved_state_that_an_update_moved_on():
+    """The convolution keeps its initial state for the backward pass: after an update of that tensor in place there is no
+    such state any more and backward says so; an update into another tensor leaves it."""
+    x, w, tok = torch.randn(2, 6, 9, device="cuda"), torch.randn(6, 4, device="cuda", requires_grad=True), torch.randn(2, 6, device="cuda")
+    state = torch.randn(2, 6, 3, device="cuda")
+    kept = state.clone()
+    run = lambda: sequence.causal_conv1d(x, w, initial_state=state, activation="silu").sum()
+    want, = torch.autograd.grad(run(), w)
+    loss = run()
+    with torch.no_grad():
+        sequence.causal_conv1d_update(tok, state, w, state_out=torch.empty_like(state))
+    assert torch.equal(torch.autograd.grad(loss, w)[0], want) and torch.equal(state, kept)
+    loss = run()
+    with torch.no_grad():
+        sequence.causal_conv1d_update(tok, state, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, w)
+    # a graph of torch's own that saved the scan's state
+    h = torch.randn(2, 6, 8, device="cuda")
+    c = torch.randn(2, 6, 8, device="cuda", requires_grad=True)
+    loss = (h * c).sum()
+    args = (tok, tok, -torch.rand(6, 8, device="cuda"), *[torch.randn(2, 1, 8, device="cuda")] * 2)
+    sequence.selective_scan_update(h, *args)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                          # tensors without a version
+        h1 = h.clone()
+        y = sequence.selective_scan_update(h1, *args)
+    assert torch.equal(sequence.selective_scan_update(h, *args), y) and torch.equal(h, h1)

@@ -256,3 +256,28 @@ def test_update_does_not_write_into_a_leaf(fake):
     with pytest.raises(RuntimeError, match="inference only"):
         sequence.selective_scan_update(fake(2, 6, 8), fake(2, 6), fake(2, 6), fake(6, 8), fake(2, 1, 8), fake(2, 1, 8),
                                        state_out=fake(2, 6, 8).requires_grad_(True))
+
+
+# ---- what an update writes to is known to autograd --------------------------------------------------------------------
+def test_updates_move_the_version_counter(fake, monkeypatch):
+    """The state is written through its address: the tensor's version moves as with any in-place operation of torch, the
+    state's own only where it is what is written."""
+    calls = []
+    monkeypatch.setattr(sequence, "_call", lambda name, *args: calls.append(name))
+    conv = lambda s, **kw: sequence.causal_conv1d_update(fake(2, 6), s, fake(6, 4), **kw)
+    scan = lambda s, **kw: sequence.selective_scan_update(s, fake(2, 6), fake(2, 6), fake(6, 8), fake(2, 1, 8), fake(2, 1, 8), **kw)
+    for update, shape in ((conv, (2, 6, 3)), (scan, (2, 6, 8))):
+        s, o = fake(*shape), fake(*shape)
+        whole = fake(2, *shape)
+        update(s)
+        assert s._version == 1
+        update(s, state_out=o)
+        assert s._version == 1 and o._version == 1
+        update(whole[1])                                                  # a view: the tensor it is a part of was written to
+        assert whole._version == 1
+        with torch.inference_mode():
+            update(fake(*shape))
+    assert len(calls) == 8
+    empty = fake(0, 6, 3)
+    sequence.causal_conv1d_update(fake(0, 6), empty, fake(6, 4))
+    assert empty._version == 0 and len(calls) == 8
