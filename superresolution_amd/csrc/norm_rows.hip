@@ -10,6 +10,10 @@
 // holding NV vectors of 16 bytes of it in registers: x (and dy) are read once, the two statistics are two butterfly
 // sums over the LPR lanes.  Bound by HBM: 2 (forward) or 3 (backward) times the tensor.
 //
+// The mean is summed relative to the row's first value: of a flat row every difference is an exact zero, so its mean is its
+// value and its variance zero.  (The sum of the values themselves is a rounded one: 96 values of 1000.1 fp32 came to a mean
+// 6e-5 off, which 1 / sqrt(eps) makes 0.02 of.)  A row's own spread bounds the differences' roundings in any case.
+//
 // A row whose length is no multiple of the vector ends in a vector that is pulled back to the row's end: its first
 // values are the neighbour's last ones again, left out of every sum and stored twice with the same bits.
 // Forward 134 us for 1048576 x 96 fp32 (6.0 TB/s), 13.4 us for 131072 x 96 bf16 (3.8 TB/s: launch and fill count there),
@@ -59,12 +63,13 @@ norm_rows_fwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
         row_vec<VEC>(lane + j * LPR, C, &start[j], &dup[j]);
         raw[j].load(xr + start[j]);
     }
+    const float first = Store<T>::get(xr[0]);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s += i >= dup[j] ? raw[j].get(i) : 0.f;
+        for (int i = 0; i < VEC; ++i) s += i >= dup[j] ? raw[j].get(i) - first : 0.f;
     const float invC = 1.0f / (float)C;
-    const float mu = row_sum<LPR>(s, red) / (float)C;         // (a division: a flat row's mean is its value)
+    const float mu = fmaf(row_sum<LPR>(s, red), invC, first);
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -120,8 +125,10 @@ norm_rows_bwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
 
     const int64_t step = (int64_t)gridDim.x * RPB;
     Raw<T, VEC> rx[NV], rd[NV], nx[NV], nd[NV];
+    T nfirst;
     auto fetch = [&](int64_t row0) {                                       // the next row is on its way while one is worked on
         const int64_t row = row0 + grp, base = (row < rows ? row : rows - 1) * C;
+        nfirst = x[base];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             nx[j].load(x + base + start[j]);
@@ -135,13 +142,14 @@ norm_rows_bwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
         const int64_t base = row * C;
 #pragma unroll
         for (int j = 0; j < NV; ++j) { rx[j] = nx[j]; rd[j] = nd[j]; }
+        const float first = Store<T>::get(nfirst);
         if (row0 + step < rows) fetch(row0 + step);
         float s = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s += i >= dup[j] ? rx[j].get(i) : 0.f;
-        const float mu = row_sum<LPR>(s, red) / (float)C;         // (a division: a flat row's mean is its value)
+            for (int i = 0; i < VEC; ++i) s += i >= dup[j] ? rx[j].get(i) - first : 0.f;
+        const float mu = fmaf(row_sum<LPR>(s, red), invC, first);
         float q = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)

@@ -671,3 +671,24 @@ def test_a_saved_state_that_an_update_moved_on():
         h1 = h.clone()
         y = sequence.selective_scan_update(h1, *args)
     assert torch.equal(sequence.selective_scan_update(h, *args), y) and torch.equal(h, h1)
+
+
+# what is flat stays flat: the values are no short binary fractions, so that the sum of a row's values is a rounded one
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [3, 7, 40, 96, 181, 400, 1030, 4099, 8192])
+def test_layernorm_flat_rows_of_any_value(C, dtype):
+    """A row of one value: its mean is that value and its variance zero, so the norm is the bias, and dx and dw too are
+    what a zero leaves: dx = r (g - mean g), dw = 0."""
+    g = _gen(C)
+    x = torch.tensor([0.1, 1000.1, -3.3e5, 7e-20, 1 / 3, -2.7]).to(dtype)[:, None].expand(6, C).contiguous()
+    w, b, dy = _uni(g, 0.5, 1.5, C), _rand(g, C), _rand(g, 6, C, dtype=dtype)
+    xg, wg, bg = _leaf(x), _leaf(w), _leaf(b)
+    y = sequence.layernorm(xg, wg, bg, 1e-5)
+    y.backward(dy.cuda())
+    assert torch.equal(y, bg.detach().to(dtype).expand(6, C))
+    assert not wg.grad.any()
+    want, mag = so.norm(torch.zeros_like(x), w, b, 1e-5, dy)
+    so.within(xg.grad, want["dx"], mag["dx"], 2 * C + 32, "dx")
+    free = sequence.layernorm(xg.detach(), wg.detach(), None, 1e-5)      # x r w, r = 1 / sqrt(eps)
+    want, mag = so.norm(x.double(), w, None, 1e-5)
+    so.within(free, want["y"], x.double().abs() * 1e-5 ** -0.5 * w.abs(), 8, "bias-free")
