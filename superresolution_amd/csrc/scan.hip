@@ -300,9 +300,12 @@ scan_chunk_kernel(const Scan a) {
 // chain the runs through LDS and walk their run again: four waves with up to 8 chunks each, or 16 with 16; what a run of that
 // length reads stays in registers for the second walk: 5.7 us for 32 chunks of 8 x 384 channels, 8.4 for 256 of 192.  (Chained in front of every chunk by the scan's own blocks, the
 // states are read as often as there are chunks: 503 MB from the caches for 256 chunks of 192 channels, 45 us instead of 20.)
-// A state of zero stays zero over a chunk whose decay overflows (growing states, A > 0): 0 times infinity is no number.
+// A chunk's decay leaves the range of fp32 where the states on both sides of it need not (1e30 times e^-100, or a growing state,
+// A > 0, of 1e-30 times e^100): it is applied as its square root, twice.  A state of zero stays zero over any growth: 0 times
+// infinity is no number.
 __device__ __forceinline__ float over_chunk(float h, float sum, float A, float own) {
-    return h == 0.f ? own : fmaf(__builtin_amdgcn_exp2f(sum * A), h, own);
+    const float root = __builtin_amdgcn_exp2f(0.5f * sum * A);
+    return h == 0.f ? own : fmaf(root * h, root, own);
 }
 template <bool REV, int RUNS, int LEN>
 __global__ void __launch_bounds__(64 * RUNS)

@@ -692,3 +692,33 @@ def test_layernorm_flat_rows_of_any_value(C, dtype):
     free = sequence.layernorm(xg.detach(), wg.detach(), None, 1e-5)      # x r w, r = 1 / sqrt(eps)
     want, mag = so.norm(x.double(), w, None, 1e-5)
     so.within(free, want["y"], x.double().abs() * 1e-5 ** -0.5 * w.abs(), 8, "bias-free")
+
+
+def _scan_against(c, softplus, dy, dlast, n, sums):
+    """Forward and backward against the oracle, n roundings to a token's result and `sums` more to a sum over tokens."""
+    want, mag = so.scan(*_scan_args(c), c["z"], c["delta_bias"], softplus, c["h0"], dy, dlast)
+    leaves = {k: _leaf(v) for k, v in c.items()}
+    out = sequence.selective_scan(*_scan_args(leaves), z=leaves["z"], delta_bias=leaves["delta_bias"], delta_softplus=softplus,
+                                  initial_state=leaves["h0"], return_last_state=True)
+    torch.autograd.backward(out, [dy.cuda(), dlast.cuda()])
+    so.within(out[0], want["y"], mag["y"], n, "y")
+    so.within(out[1], want["last"], mag["last"], n, "last")
+    for k, v in leaves.items():
+        if v is not None:
+            so.within(v.grad, want["d" + k], mag["d" + k], n if v.dim() == 3 and k != "h0" else n + sums, "d" + k)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_selective_scan_states_that_cross_the_range_of_a_decay(sign):
+    """The decay of 48 tokens together, e^(+-144), does not fit fp32, the states on both sides of them do: 1e-30 grows to
+    3e32, or 1e30 falls to 1e-33.  The rounded exponents of a token are below 5, so that 8 roundings a token cover them.
+    (The inputs are small throughout: a state of 1e30 that meets a gradient of 1e30 would have a step size's gradient of 1e60.)"""
+    g = _gen(15)
+    B, D, N, L = 2, 5, 4, 900
+    first = 1e-30 if sign > 0 else 1e30
+    c = dict(x=_rand(g, B, D, L, scale=1e-30), A=sign * torch.ones(D, N), B=_rand(g, B, 1, N, L), C=_rand(g, B, 1, N, L), D=None, z=None,
+             delta_bias=None, h0=_uni(g, 1.0, 2.0, B, D, N) * first)
+    c["delta"] = torch.zeros(B, D, L)
+    c["delta"][..., 96:144] = 3.0
+    dy, dlast = _rand(g, B, D, L, scale=1e-30 if sign > 0 else 1e-3), _uni(g, 1.0, 2.0, B, D, N) * first
+    _scan_against(c, False, dy, dlast, 8 * L + N + D + B + 80, 0)
