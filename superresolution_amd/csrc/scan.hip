@@ -181,10 +181,16 @@ __device__ __forceinline__ ScanTile scan_tile(const Scan& a, const ScanPlace& p,
 
 __device__ __forceinline__ float step_size(const Scan& a, float raw) { return a.softplus ? softplus(raw) : raw; }
 
-// A (times log2 e) of the lane's channel and four states; zero where there are none, so that they stay zero
+// A rate is at most 2^100: an infinite one (a state without memory) times a step size of zero is no number, and such a token, in
+// padding or behind the row's end in a tile, has to leave the state alone, and to have a gradient of zero (the rate times a
+// state and its gradient must not overflow).  2^100 times any step size above 1e-28 decays as infinity does.
+__device__ __forceinline__ float finite_rate(float A) {
+    return fabsf(A) > 0x1p100f ? copysignf(0x1p100f, A) : A;               // (what is no number stays so)
+}
+// A of the lane's channel and four states; zero where there are none, so that they stay zero
 __device__ __forceinline__ void load_rates(const Scan& a, int d, bool ok, int wave, float (&A)[4]) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) A[s] = ok && wave * 4 + s < a.N ? a.A[(int64_t)d * a.N + wave * 4 + s] : 0.f;
+    for (int s = 0; s < 4; ++s) A[s] = ok && wave * 4 + s < a.N ? finite_rate(a.A[(int64_t)d * a.N + wave * 4 + s]) : 0.f;
 }
 
 // dt of four tokens: zero where there is no channel (all: the block has 64) or token, so that nothing there moves a state
@@ -315,7 +321,7 @@ scan_chain_kernel(const Scan a, int states) {
     const int d = blockIdx.x * 64 + lane, n = blockIdx.y, b = blockIdx.z;
     const bool ok = d < a.D;
     const int dr = ok ? d : 0;
-    const float A = n < a.N ? a.A[(int64_t)dr * a.N + n] * LOG2E : 0.f;
+    const float A = n < a.N ? finite_rate(a.A[(int64_t)dr * a.N + n]) * LOG2E : 0.f;
     const int per = (a.nchunk + RUNS - 1) / RUNS, c0 = run * per, c1 = c0 + per < a.nchunk ? c0 + per : a.nchunk;
     float* st = a.cst + ((int64_t)b * a.nchunk * states + n) * a.D;        // chunk c: + c states D
     const float* dt = a.cdt + (int64_t)b * a.nchunk * a.D;
@@ -799,7 +805,7 @@ scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const f
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (n0 + k < N) {
-                h[k] = fmaf(exp_fast(dt * Av[k]), h[k], u * Store<T>::get(Bm[bg * N + n0 + k]));
+                h[k] = fmaf(exp_fast(dt * finite_rate(Av[k])), h[k], u * Store<T>::get(Bm[bg * N + n0 + k]));
                 s = fmaf(Store<T>::get(Cm[bg * N + n0 + k]), h[k], s);
             }
         if ((N & 3) == 0 && n0 < N) {

@@ -722,3 +722,30 @@ def test_selective_scan_states_that_cross_the_range_of_a_decay(sign):
     c["delta"][..., 96:144] = 3.0
     dy, dlast = _rand(g, B, D, L, scale=1e-30 if sign > 0 else 1e-3), _uni(g, 1.0, 2.0, B, D, N) * first
     _scan_against(c, False, dy, dlast, 8 * L + N + D + B + 80, 0)
+
+
+@pytest.mark.parametrize("L", [16, 21, 45])
+def test_selective_scan_states_without_memory(L):
+    """A rate of -inf forgets a state at every token; at a token whose step size is zero, behind the row's end in a tile as in
+    padding, even such a state stays as it is."""
+    g = _gen(16)
+    c = _scan_case(g, 2, 6, 2, 5, L, F32, True, True, True)
+    c["A"][:, 0] = -float("inf")
+    dev = {k: v.cuda() for k, v in c.items()}
+    kw = dict(z=dev["z"], delta_bias=dev["delta_bias"], delta_softplus=True, return_last_state=True)
+    want, mag = so.scan(*_scan_args(c), c["z"], c["delta_bias"], True, c["h0"])
+    y, last = sequence.selective_scan(*_scan_args(dev), initial_state=dev["h0"], **kw)
+    so.within(y, want["y"], mag["y"], 8 * L + 100, "y")
+    so.within(last, want["last"], mag["last"], 8 * L + 100, "last")
+    dev["delta"] = torch.full_like(dev["delta"], -float("inf"))
+    leaves = {k: v.clone().requires_grad_(True) for k, v in dev.items()}
+    kw.update(z=leaves["z"], delta_bias=leaves["delta_bias"])
+    y, held = sequence.selective_scan(*_scan_args(leaves), initial_state=leaves["h0"], **kw)
+    assert torch.equal(held, dev["h0"])
+    held.sum().backward()
+    assert torch.equal(leaves["h0"].grad, torch.ones_like(dev["h0"])) and not leaves["delta"].grad.any() and not leaves["A"].grad.any()
+    state = dev["h0"].clone()
+    one = lambda k: dev[k][..., 0]
+    sequence.selective_scan_update(state, one("x"), one("delta"), dev["A"], one("B"), one("C"), dev["D"], delta_bias=dev["delta_bias"],
+                                   delta_softplus=True)
+    assert torch.equal(state, dev["h0"])
