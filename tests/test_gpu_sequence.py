@@ -749,3 +749,18 @@ def test_selective_scan_states_without_memory(L):
     sequence.selective_scan_update(state, one("x"), one("delta"), dev["A"], one("B"), one("C"), dev["D"], delta_bias=dev["delta_bias"],
                                    delta_softplus=True)
     assert torch.equal(state, dev["h0"])
+
+
+@pytest.mark.parametrize("B,L", [(1, 17000), (2, 24000)])
+def test_selective_scan_many_chunks(B, L):
+    """More chunks than a run of the chain keeps in registers (355 both ways, and 375 forward for two samples), with states
+    that reach over several of them.  All terms are positive and between 0.6 and 1.7 of their usual size, so a
+    rounding of a term of age k, of which there are 8 k, weighs a^k of it: with a <= exp(-0.018) the ages come to 56 tokens, and
+    8 x 56 x (1.7 / 0.6) = 1270 roundings stand for any result of a token; the products of the backward pass have twice as many.
+    A parameter's gradient adds a rounding a token and sample."""
+    g = _gen(17)
+    D, N = 8, 4
+    u = lambda *shape: _uni(g, 0.9, 1.1, *shape)
+    c = dict(x=u(B, D, L), delta=0.2 * u(B, D, L), A=-_uni(g, 0.1, 0.5, D, N), B=u(B, 1, N, L), C=u(B, 1, N, L), D=u(D), z=None,
+             delta_bias=None, h0=10 * u(B, D, N))
+    _scan_against(c, False, u(B, D, L), 10 * u(B, D, N), 2 * 1270 + N + D + 80, B * L)
