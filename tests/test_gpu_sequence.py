@@ -764,3 +764,29 @@ def test_selective_scan_many_chunks(B, L):
     c = dict(x=u(B, D, L), delta=0.2 * u(B, D, L), A=-_uni(g, 0.1, 0.5, D, N), B=u(B, 1, N, L), C=u(B, 1, N, L), D=u(D), z=None,
              delta_bias=None, h0=10 * u(B, D, N))
     _scan_against(c, False, u(B, D, L), 10 * u(B, D, N), 2 * 1270 + N + D + 80, B * L)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("C", [96, 513, 1000, 1536, 2048, 4096, 8192])
+def test_layernorm_long_rows_lose_no_bits(C, bias, dtype):
+    """The sums over a row are trees: at most 32 values of a lane one by one, then 9 steps over the lanes, 41 roundings and not
+    C.  With the differences, the division and the square root 2 x 41 + 46 = 128 roundings lie between an input and y; the
+    magnitudes count the row's first value beside the mean, since either may be what the others are taken relative to.  dx
+    and dw have the products of two such factors."""
+    g = _gen(C)
+    x, dy = _rand(g, 5, C, dtype=dtype, shift=0.5), _rand(g, 5, C, dtype=dtype)
+    w, b = _uni(g, 0.5, 1.5, C), _rand(g, C, scale=0.1) if bias else None
+    xg, wg, bg = _leaf(x), _leaf(w), _leaf(b)
+    y = sequence.layernorm(xg, wg, bg, 1e-5)
+    y.backward(dy.cuda())
+    want = so.norm(x, w, b, 1e-5, dy)[0]
+    xd, gd = x.double(), (dy.double() * w).abs()
+    mean = lambda t: t.mean(-1, keepdim=True)
+    r = 1 / torch.sqrt(xd.var(-1, unbiased=False, keepdim=True) + 1e-5)
+    wide = (xd.abs() + mean(xd.abs()) + xd[:, :1].abs()) * r
+    so.within(y, want["y"], wide * w + (b.double().abs() if bias else 0), 128, "y")
+    so.within(xg.grad, want["dx"], r * (gd + mean(gd) + wide * mean(gd * wide) * (1 if bias else 2)), 256, "dx")
+    so.within(wg.grad, want["dw"], (dy.double().abs() * wide).sum(0), 133, "dw")
+    if bias:
+        so.within(bg.grad, want["db"], dy.double().abs().sum(0), 13, "db")
