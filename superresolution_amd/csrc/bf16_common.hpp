@@ -10,10 +10,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {     // round to nearest even
-    uint32_t r;
-    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
-    return r;
+// Round to nearest even: v_cvt_pk_bf16_f32.  A conversion that the compiler sees, not inline assembly, so that it keeps the wait
+// states between this write and a lane exchange that reads it (v_permlane16_swap, DPP: two).
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
 }
 __device__ __forceinline__ void unpack8(const u32x4 w, float* v) {
 #pragma unroll
