@@ -269,7 +269,10 @@ attn_bwd_wo_kernel(const float* __restrict__ P, const float* __restrict__ attn, 
     const int tid = threadIdx.x;
     const int m0 = blockIdx.x * 16, h = blockIdx.y, b = blockIdx.z;
     const float* Abh = attn + ((int64_t)b * heads + h) * c * c;
+    // (several loads in flight: one at a time costs a bf16 training step 0.59 ms here instead of 0.47)
+#pragma unroll 8
     for (int e = tid; e < c * c; e += 256) As[(e / c) * (c + 1) + (e % c)] = Abh[e];
+#pragma unroll 4
     for (int e = tid; e < 16 * c; e += 256) {
         const int r = e / c, j = e % c;
         Ps[e] = (m0 + r < C) ? P[((int64_t)b * C + m0 + r) * C + h * c + j] : 0.f;

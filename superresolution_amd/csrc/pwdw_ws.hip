@@ -1,8 +1,6 @@
 // Host side of the wave-specialised fused 1x1 + depthwise kernels (pwdw_ws_kernel.hpp) and the plain
-// instantiation.  This file is compiled WITH packing of adjacent scalar float operations into v_pk_* (the
-// vector waves' depthwise arithmetic halves its instruction count, and the kernel is bound by the total
-// instruction issue of a SIMD); the gated instantiation lives in pwdw_ws_gate.hip, compiled without it
-// (packed temporaries push its 128-register vector waves into spilling).
+// instantiation.  The gated instantiation lives in pwdw_ws_gate.hip and is compiled without the compiler's pairing of adjacent
+// scalar float operations, whose temporaries push its 128-register vector waves into spilling.
 #include "pwdw_ws_kernel.hpp"
 
 
