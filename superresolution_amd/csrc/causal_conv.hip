@@ -44,7 +44,7 @@ struct CausalConv {
 // the row and segment of this lane's group of TX lanes
 template <int TX>
 __device__ __forceinline__ bool conv_place(const CausalConv& a, int64_t* row, int* seg, int* lane) {
-    uint32_t item = blockIdx.x * (256 / TX) + threadIdx.x / TX;          // rows x segments < 2^31: causal_conv_plan
+    uint32_t item = block_index<256>() * (256 / TX) + threadIdx.x / TX;         // rows x segments < 2^31: causal_conv_plan
     if (TX == 64) item = __builtin_amdgcn_readfirstlane(item);           // one row to a wave: its weights are scalar loads
     *lane = threadIdx.x % TX;
     *seg = (int)(item % (uint32_t)a.nseg);
@@ -106,7 +106,7 @@ causal_conv_fwd_kernel(const CausalConv a) {
 template <typename T, int W>
 __global__ void __launch_bounds__(256)
 causal_conv_fwd_short_kernel(const CausalConv a) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = (int64_t)block_index<256>() * 256 + threadIdx.x;
     if (row >= (int64_t)a.B * a.D) return;
     const int d = (int)(row % a.D), L = (int)a.L;
     const ConvRow<T> in{static_cast<const T*>(a.x) + row * a.L,
@@ -232,7 +232,7 @@ causal_conv_bwd_kernel(const CausalConv a) {
 template <typename T, int W>
 __global__ void __launch_bounds__(256)
 causal_conv_bwd_short_kernel(const CausalConv a) {
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = (int64_t)block_index<256>() * 256 + threadIdx.x;
     if (row >= (int64_t)a.B * a.D) return;
     const int d = (int)(row % a.D), L = (int)a.L;
     const ConvRow<T> in{static_cast<const T*>(a.x) + row * a.L,
@@ -278,8 +278,9 @@ template <int W>
 __global__ void __launch_bounds__(256)
 causal_conv_reduce_kernel(const float* __restrict__ partial, int n, int D, float* __restrict__ dw, float* __restrict__ db) {
     __shared__ float red[32][CC_PART + 1];
-    const int d = blockIdx.x, k = threadIdx.x % CC_PART, slice = threadIdx.x / CC_PART;
+    const int d = (int)block_index<256>(), k = threadIdx.x % CC_PART, slice = threadIdx.x / CC_PART;
     float s = 0.f;
+    if (d >= D) return;
     if (k <= W)
         for (int64_t p = slice; p < n; p += 32) s += partial[(p * D + d) * CC_PART + k];
     red[slice][k] = s;
@@ -299,7 +300,7 @@ template <typename T, int W>
 __global__ void __launch_bounds__(256)
 causal_conv_update_kernel(const T* __restrict__ x, const T* state, T* state_out, const float* __restrict__ w,
                           const float* __restrict__ b, T* __restrict__ y, int64_t n, int D, int act) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (int64_t)block_index<256>() * 256 + threadIdx.x;
     if (i >= n) return;
     const int d = (int)(i % D);
     T in[W];
@@ -338,11 +339,11 @@ static int causal_conv_fwd_t(CausalConv a, hipStream_t st) {
     const int64_t rows = (int64_t)a.B * a.D;
     ProfScope prof(st, "causal_conv_fwd", (2.0 * W + 5) * rows * a.L, 2.0 * sizeof(T) * rows * a.L);
     if (a.L < CC_TOK) {
-        hipLaunchKernelGGL((causal_conv_fwd_short_kernel<T, W>), dim3((unsigned)cdiv(rows, 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((causal_conv_fwd_short_kernel<T, W>), grid_of<256>(cdiv(rows, 256)), dim3(256), 0, st, a);
     } else if (causal_conv_plan(&a) == 64) {
-        hipLaunchKernelGGL((causal_conv_fwd_kernel<T, W, 64>), dim3((unsigned)cdiv(rows * a.nseg, 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((causal_conv_fwd_kernel<T, W, 64>), grid_of<256>(cdiv(rows * a.nseg, 4)), dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL((causal_conv_fwd_kernel<T, W, 8>), dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((causal_conv_fwd_kernel<T, W, 8>), grid_of<256>(cdiv(rows, 32)), dim3(256), 0, st, a);
     }
     RST_LAUNCH_CHECK();
     return RST_OK;
@@ -354,14 +355,14 @@ static int causal_conv_bwd_t(CausalConv a, float* dw, float* db, hipStream_t st)
     ProfScope prof(st, "causal_conv_bwd", (6.0 * W + 10) * rows * a.L, 3.0 * sizeof(T) * rows * a.L);
     if (a.L < CC_TOK) {
         a.nseg = 1;
-        hipLaunchKernelGGL((causal_conv_bwd_short_kernel<T, W>), dim3((unsigned)cdiv(rows, 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((causal_conv_bwd_short_kernel<T, W>), grid_of<256>(cdiv(rows, 256)), dim3(256), 0, st, a);
     } else if (causal_conv_plan(&a) == 64) {
-        hipLaunchKernelGGL((causal_conv_bwd_kernel<T, W, 64>), dim3((unsigned)cdiv(rows * a.nseg, 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((causal_conv_bwd_kernel<T, W, 64>), grid_of<256>(cdiv(rows * a.nseg, 4)), dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL((causal_conv_bwd_kernel<T, W, 8>), dim3((unsigned)cdiv(rows, 32)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((causal_conv_bwd_kernel<T, W, 8>), grid_of<256>(cdiv(rows, 32)), dim3(256), 0, st, a);
     }
     RST_LAUNCH_CHECK();
-    hipLaunchKernelGGL((causal_conv_reduce_kernel<W>), dim3((unsigned)a.D), dim3(256), 0, st, a.partial, a.B * a.nseg, a.D, dw, db);
+    hipLaunchKernelGGL((causal_conv_reduce_kernel<W>), grid_of<256>(a.D), dim3(256), 0, st, a.partial, a.B * a.nseg, a.D, dw, db);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
@@ -370,7 +371,7 @@ template <typename T, int W>
 static int causal_conv_update_t(const T* x, const T* state, T* state_out, const float* w, const float* b, T* y, int64_t n, int D, int act,
                                 hipStream_t st) {
     ProfScope prof(st, "causal_conv_update", (2.0 * W + 5) * n, 2.0 * W * sizeof(T) * n);
-    hipLaunchKernelGGL((causal_conv_update_kernel<T, W>), dim3((unsigned)cdiv(n, 256)), dim3(256), 0, st, x, state, state_out, w, b, y, n,
+    hipLaunchKernelGGL((causal_conv_update_kernel<T, W>), grid_of<256>(cdiv(n, 256)), dim3(256), 0, st, x, state, state_out, w, b, y, n,
                        D, act);
     RST_LAUNCH_CHECK();
     return RST_OK;

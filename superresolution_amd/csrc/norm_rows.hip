@@ -52,7 +52,7 @@ norm_rows_fwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
                      T* __restrict__ y, int64_t rows, int C, float eps) {
     __shared__ float red[4];
     const int lane = threadIdx.x % LPR;
-    const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int64_t row = (int64_t)block_index<256>() * (256 / LPR) + threadIdx.x / LPR;
     const bool live = row < rows;
     const T* xr = x + (live ? row : 0) * C;
     Raw<T, VEC> raw[NV];
@@ -285,7 +285,7 @@ static constexpr bool nr_reached(int vec, int lpr, int nv) {
 #define NR_DISPATCH(KERNEL, LDS, GRID, ...)                                                                               \
     do {                                                                                                                \
         if (p.vec == 1) {                                                                                                 \
-            hipLaunchKernelGGL((KERNEL<T, 1, 8, 1>), dim3((unsigned)(GRID)), dim3(256), LDS, st, __VA_ARGS__);             \
+            hipLaunchKernelGGL((KERNEL<T, 1, 8, 1>), grid_of<256>(GRID), dim3(256), LDS, st, __VA_ARGS__);             \
         } else switch (p.lpr * 16 + p.nv) {                                                                              \
             NR_CASES(NR_CASE_OF, KERNEL, LDS, GRID, __VA_ARGS__)                                                          \
             default: return fail(RST_ERR_INVALID, "rows_norm: no kernel for C=%d", C);                                    \
@@ -295,7 +295,7 @@ static constexpr bool nr_reached(int vec, int lpr, int nv) {
 #define NR_CASE_OF(L_, N_, KERNEL, LDS, GRID, ...)                                                                        \
     case L_ * 16 + N_:                                                                                                   \
         if constexpr (nr_reached(V, L_, N_))                                                                         \
-            hipLaunchKernelGGL((KERNEL<T, V, L_, N_>), dim3((unsigned)(GRID)), dim3(256), LDS, st, __VA_ARGS__);          \
+            hipLaunchKernelGGL((KERNEL<T, V, L_, N_>), grid_of<256>(GRID), dim3(256), LDS, st, __VA_ARGS__);          \
         break;
 
 template <typename T>

@@ -60,9 +60,9 @@ __device__ __forceinline__ float softplus(float v) {
 // which chunk, sample, group and channels a block has
 struct ScanPlace {
     int b, g, cb, chunk, lane, wave;
-    __device__ __forceinline__ ScanPlace(const Scan& a, int chunks, int first) {
+    __device__ __forceinline__ ScanPlace(const Scan& a, uint32_t block, int chunks, int first) {
         const uint32_t per = (uint32_t)(a.G * a.cb);
-        uint32_t i = blockIdx.x;
+        uint32_t i = block;
         const uint32_t gc = i % per;
         i /= per;
         chunk = (int)(i % (uint32_t)chunks) + first;
@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(64 * W, 8)                               // (a
 scan_chunk_kernel(const Scan a) {
     constexpr int NI = ScanItems<W>::N;
     __shared__ float dts[ST][SROW], us[ST][SROW];
-    const ScanPlace p(a, a.nchunk - 1, REV ? 1 : 0);
+    const ScanPlace p(a, block_index<64 * W>(), a.nchunk - 1, REV ? 1 : 0);
+    if (p.b >= a.B) return;
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
     const bool ok = p.cb * SC + p.lane < a.Dg;
     const bool whole = p.cb * SC + SC <= a.Dg;
@@ -379,7 +380,8 @@ __global__ void __launch_bounds__(64 * W, 6)
 scan_fwd_kernel(const Scan a) {
     constexpr int NI = ScanItems<W>::N;
     __shared__ __attribute__((aligned(16))) float dts[ST][SROW], us[ST][SROW], part[W][ST][SROW];
-    const ScanPlace p(a, a.nchunk, 0);
+    const ScanPlace p(a, block_index<64 * W>(), a.nchunk, 0);
+    if (p.b >= a.B) return;
     const int d = p.g * a.Dg + p.cb * SC + p.lane;
     const bool ok = p.cb * SC + p.lane < a.Dg, whole = p.cb * SC + SC <= a.Dg;
     const int64_t bg = (int64_t)p.b * a.G + p.g;
@@ -715,7 +717,8 @@ template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)                  // (fewer waves have more tokens a lane: 256 registers would spill)
 scan_bwd_kernel(const Scan a) {
     extern __shared__ __attribute__((aligned(16))) float smem[];
-    const ScanPlace p(a, a.nchunk, 0);
+    const ScanPlace p(a, block_index<64 * W>(), a.nchunk, 0);
+    if (p.b >= a.B) return;
     if (p.cb * SC + SC <= a.Dg) scan_bwd_body<T, W, Z, true>(a, p, smem);
     else scan_bwd_body<T, W, Z, false>(a, p, smem);
 }
@@ -727,10 +730,11 @@ scan_bwd_kernel(const Scan a) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 scan_reduce_kernel(const Scan a, int W, int bcs, float* __restrict__ dA, float* __restrict__ dD, float* __restrict__ dbias) {
-    if (blockIdx.x < (unsigned)bcs) {
+    const uint32_t block = block_index<256>();
+    if (block < (uint32_t)bcs) {
         const int across = (int)((a.L + 63) / 64);
-        const int64_t t = (int64_t)(blockIdx.x % across) * 64 + (threadIdx.x & 63);
-        const int64_t bg = blockIdx.x / across, groups = (int64_t)a.tiles * 2, stride = (int64_t)a.B * a.G * groups * W * 64;
+        const int64_t t = (int64_t)(block % across) * 64 + (threadIdx.x & 63);
+        const int64_t bg = block / across, groups = (int64_t)a.tiles * 2, stride = (int64_t)a.B * a.G * groups * W * 64;
         if (t >= a.L) return;
         T *dB = static_cast<T*>(a.dB), *dC = static_cast<T*>(a.dC);
         for (int n = threadIdx.x >> 6; n < a.N; n += 4) {
@@ -747,8 +751,9 @@ scan_reduce_kernel(const Scan a, int W, int bcs, float* __restrict__ dA, float* 
     }
     __shared__ float red[16][17];
     const int col = threadIdx.x & 15, slice = threadIdx.x >> 4, wide = (a.D + 15) / 16;
-    const int i = blockIdx.x - bcs, d = i % wide * 16 + col, row = i / wide, n = a.B * a.nchunk;
+    const int i = (int)(block - bcs), d = i % wide * 16 + col, row = i / wide, n = a.B * a.nchunk;
     float s = 0.f;
+    if (row > a.N + 1) return;
     if (d < a.D) {
         const float* p = row < a.N ? a.dApart + (int64_t)row * a.D + d : a.dDpart + (int64_t)(row - a.N) * a.D + d;
         const int64_t step = (int64_t)(row < a.N ? 4 * W : 2) * a.D;
@@ -776,7 +781,7 @@ scan_update_kernel(const T* __restrict__ x, const T* __restrict__ delta, const f
                    const T* __restrict__ Cm, const float* __restrict__ Dskip, const T* __restrict__ z,
                    const float* __restrict__ dbias, const float* state, float* state_out, T* __restrict__ y, int64_t n, int D, int G,
                    int N, int soft) {
-    const int64_t i = (int64_t)blockIdx.x * (256 / NL) + threadIdx.x / NL;
+    const int64_t i = (int64_t)block_index<256>() * (256 / NL) + threadIdx.x / NL;
     const int lane = threadIdx.x % NL;
     const bool live = i < n;
     float s = 0.f, xv = 0.f;
@@ -917,11 +922,11 @@ static int scan_fwd_t(const Scan& a, hipStream_t st) {
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, false, false>), grid_of<64 * W>(per * (a.nchunk - 1)), dim3(64 * W), 0, st, a);
         RST_LAUNCH_CHECK();
         RST_TRY(scan_chain<false>(a, 4 * W, st));
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), 0, st, a);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, W, Z>), grid_of<64 * W>(per * a.nchunk), dim3(64 * W), 0, st, a);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
@@ -933,18 +938,18 @@ static int scan_bwd_t(const Scan& a, float* dA, float* dD, float* dbias, hipStre
     const int64_t per = (int64_t)a.B * a.G * a.cb;
     RST_REQUIRE(per * a.nchunk < (1ll << 31), "scan: grid out of range");
     if (a.nchunk > 1) {
-        hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), dim3((unsigned)(per * (a.nchunk - 1))), dim3(64 * W), 0, st, a);
+        hipLaunchKernelGGL((scan_chunk_kernel<T, W, Z, true>), grid_of<64 * W>(per * (a.nchunk - 1)), dim3(64 * W), 0, st, a);
         RST_LAUNCH_CHECK();
         RST_TRY(scan_chain<true>(a, 4 * W, st));
     }
     const size_t lds = (size_t)(3 + (Z ? 3 : 2) * W) * ST * SROW * sizeof(float);
     KernelSetup ks;
     RST_TRY(kernel_setup(reinterpret_cast<const void*>(scan_bwd_kernel<T, W, Z>), 64 * W, lds, &ks));
-    hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), dim3((unsigned)(per * a.nchunk)), dim3(64 * W), lds, st, a);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, W, Z>), grid_of<64 * W>(per * a.nchunk), dim3(64 * W), lds, st, a);
     RST_LAUNCH_CHECK();
     const int64_t bcs = cdiv(a.L, 64) * a.B * a.G, all = bcs + cdiv(a.D, 16) * (a.N + 2);
     RST_REQUIRE(all < (1ll << 31), "scan: grid out of range");
-    hipLaunchKernelGGL((scan_reduce_kernel<T>), dim3((unsigned)all), dim3(256), 0, st, a, W, (int)bcs, dA, dD, dbias);
+    hipLaunchKernelGGL((scan_reduce_kernel<T>), grid_of<256>(all), dim3(256), 0, st, a, W, (int)bcs, dA, dD, dbias);
     RST_LAUNCH_CHECK();
     return RST_OK;
 }
@@ -953,7 +958,7 @@ template <typename T, int NL>
 static int scan_update_t(const rst_scan_desc* s, const rst_scan_inputs* in, const float* state, float* state_out, T* y, hipStream_t st) {
     const int64_t n = (int64_t)s->B * s->D;
     ProfScope prof(st, "scan_update", n * (7.0 * s->N + 20), n * 8.0 * s->N);
-    hipLaunchKernelGGL((scan_update_kernel<T, NL>), dim3((unsigned)cdiv(n, 256 / NL)), dim3(256), 0, st, static_cast<const T*>(in->x),
+    hipLaunchKernelGGL((scan_update_kernel<T, NL>), grid_of<256>(cdiv(n, 256 / NL)), dim3(256), 0, st, static_cast<const T*>(in->x),
                        static_cast<const T*>(in->delta), in->A, static_cast<const T*>(in->B), static_cast<const T*>(in->C), in->D,
                        static_cast<const T*>(in->z), in->delta_bias, state, state_out, y, n, s->D, s->G, s->N, s->delta_softplus);
     RST_LAUNCH_CHECK();

@@ -4,6 +4,16 @@
 
 namespace rst {
 
+// A launch has fewer than 2^32 threads along x.  More blocks than that go into rows of 2^31 / THREADS blocks along y; the last
+// row then has blocks past the end, which a kernel sends home.
+template <int THREADS> static dim3 grid_of(int64_t blocks) {
+    constexpr int64_t ROW = (1ll << 31) / THREADS;
+    return blocks <= ROW ? dim3((unsigned)blocks) : dim3((unsigned)ROW, (unsigned)cdiv(blocks, ROW));
+}
+template <int THREADS> __device__ __forceinline__ uint32_t block_index() {
+    return blockIdx.y * (uint32_t)((1ll << 31) / THREADS) + blockIdx.x;
+}
+
 // Values per 16 bytes, and conversions of the two storage types.  All arithmetic is fp32; a bf16 result is rounded
 // once, to nearest even, when it is stored.
 template <typename T> struct Store;

@@ -790,3 +790,93 @@ def test_layernorm_long_rows_lose_no_bits(C, bias, dtype):
     so.within(wg.grad, want["dw"], (dy.double().abs() * wide).sum(0), 133, "dw")
     if bias:
         so.within(bg.grad, want["db"], dy.double().abs().sum(0), 13, "db")
+
+
+def test_layernorm_more_rows_than_one_row_of_blocks():
+    """2^29 rows of 8 are more than 2^24 blocks: a launch has fewer than 2^32 threads along one dimension."""
+    rows, C = (1 << 29) + 37, 8
+    x = torch.zeros(rows, C, dtype=BF16, device="cuda")
+    w, b = torch.linspace(0.5, 1.5, C, device="cuda"), torch.linspace(-1.0, 1.0, C, device="cuda")
+    places = torch.tensor([0, 31, 32, (1 << 28) - 1, 1 << 28, (1 << 29) - 1, 1 << 29, rows - 33, rows - 32, rows - 1], device="cuda")
+    x[places] = torch.randn(places.numel(), C, device="cuda").to(BF16)
+    y = sequence.layernorm(x, w, b)
+    assert torch.equal(y[places], sequence.layernorm(x[places], w, b))
+    y[places] = b.to(BF16)
+    for at in range(0, rows, 1 << 26):                       # (piece by piece: a comparison of the whole takes its size again)
+        assert (y[at:at + (1 << 26)] == b.to(BF16)).all(), at
+
+
+def test_causal_conv1d_more_channels_than_one_row_of_blocks():
+    """2^24 + 1 channels are more blocks than one row of them in the sum over the weight's shares, 32 samples of them in the
+    kernels before it."""
+    B, D, L, W = 32, (1 << 24) + 1, 8, 4
+    x, dy = torch.zeros(B, D, L, dtype=BF16, device="cuda"), torch.zeros(B, D, L, dtype=BF16, device="cuda")
+    w, b = torch.rand(D, W, device="cuda"), torch.rand(D, device="cuda")
+    at = torch.tensor([0, 1, 31, 32, (1 << 23) - 1, 1 << 23, D - 2, D - 1], device="cuda")
+    for t in (x, dy):
+        t[:, at] = torch.randn(B, at.numel(), L, device="cuda").to(BF16)
+
+    def run(x, w, b, dy):
+        ins = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = sequence.causal_conv1d(*ins, activation="silu")
+        return [y.detach(), *torch.autograd.grad(y, ins, dy)]
+    y, dx, dw, db = run(x, w, b, dy)
+    sy, sdx, sdw, sdb = run(x[:, at], w[at], b[at], dy[:, at])
+    assert torch.equal(y[:, at], sy) and torch.equal(dx[:, at], sdx) and torch.equal(dw[at], sdw) and torch.equal(db[at], sdb)
+    for t in (dw, db):
+        t[at] = 0
+        assert not t.any()
+
+
+def test_selective_scan_more_channels_than_one_row_of_blocks():
+    """65535 samples of 8256 channels and 17 states: 2^23 blocks of 512 threads, for one token of the scan and for an update."""
+    B, D, N = 65535, 8256, 17
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    A, bias = -torch.rand(D, N, generator=gen, device="cuda") - 0.1, torch.rand(D, generator=gen, device="cuda")
+    bc = torch.randn(2, B, 1, N, 1, generator=gen, device="cuda").to(BF16)
+    x, delta = torch.zeros(B, D, 1, dtype=BF16, device="cuda"), torch.zeros(B, D, 1, dtype=BF16, device="cuda")
+    at = torch.tensor([0, 1, 32767, 32768, 65000, 65533, 65534], device="cuda")
+    x[at] = torch.randn(at.numel(), D, 1, generator=gen, device="cuda").to(BF16)
+    kw = dict(delta_bias=bias, delta_softplus=True)
+    y = sequence.selective_scan(x, delta, A, bc[0], bc[1], **kw)
+    assert torch.equal(y[at], sequence.selective_scan(x[at], delta[at], A, bc[0][at], bc[1][at], **kw))
+    y[at] = 0
+    assert not y.any()
+    del y
+    state = torch.zeros(B, D, N, device="cuda")
+    small = torch.rand(at.numel(), D, N, generator=gen, device="cuda")
+    state[at] = small
+    one = lambda t: t[..., 0]
+    y = sequence.selective_scan_update(state, one(x), one(delta), A, one(bc[0]), one(bc[1]), **kw)
+    want = sequence.selective_scan_update(small, one(x)[at], one(delta)[at], A, one(bc[0])[at], one(bc[1])[at], **kw)
+    assert torch.equal(y[at], want) and torch.equal(state[at], small)
+    y[at] = 0
+    assert not y.any() and not state[30000].any()
+
+
+def test_selective_scan_more_tokens_than_one_row_of_blocks():
+    """64 samples of 2^24 tokens: 2^24 blocks for the shares of dB and dC alone.  As in the test of the longest row, nothing
+    enters a state or its gradient before a sample's last 200 tokens, and every term is positive."""
+    B, L, K = 64, sequence.MAX_TOKENS, 200
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    A = torch.tensor([[-0.7]], device="cuda")
+    x, dy = torch.zeros(B, 1, L, dtype=BF16, device="cuda"), torch.zeros(B, 1, L, dtype=BF16, device="cuda")
+    for t in (x, dy):
+        t[..., -K:] = (torch.rand(B, 1, K, generator=gen, device="cuda") + 0.5).to(BF16)
+    delta = torch.full((B, 1, L), 0.3, dtype=BF16, device="cuda")
+    bc = torch.ones(B, 1, 1, L, dtype=BF16, device="cuda")
+
+    def grads(x, delta, bc, dy):
+        ins = [t.detach().requires_grad_(True) for t in (x, bc, bc)]
+        y = sequence.selective_scan(ins[0], delta, A, ins[1], ins[2])
+        return (y.detach(),) + torch.autograd.grad(y, ins, dy)
+    whole = grads(x, delta, bc, dy)
+    cut = lambda t: t[..., -K:].contiguous()
+    end = grads(cut(x), cut(delta), cut(bc), cut(dy))
+    n = 8 * K + 83
+    for name, w, e in zip(("y", "dx", "dB", "dC"), whole, end):
+        assert e.min() > 0, name
+        err = float(((cut(w).float() - e.float()).abs() / e.float()).max())
+        assert err <= 2 * n * 2.0 ** -24 + 2 * 2.0 ** -8, (name, err)
+    for at in (0, 1, 31, 62, 63):
+        assert not whole[2][at, ..., :-K].any() and not whole[3][at, ..., :-K].any() and not whole[0][at, ..., :-K].any()
