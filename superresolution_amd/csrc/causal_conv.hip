@@ -416,7 +416,8 @@ int rst_causal_conv1d_fwd(const void* x, int32_t dtype, const float* weight, con
 }
 
 size_t rst_causal_conv1d_bwd_workspace_bytes(int32_t B, int32_t D, int64_t L) {
-    return B > 0 && D > 0 && L > 0 ? causal_conv_bwd_ws(B, D, L) : 0;
+    if (causal_conv_check("causal_conv1d_bwd_workspace_bytes", RST_DTYPE_F32, B, D, L, 2) != RST_OK) return 0;
+    return causal_conv_bwd_ws(B, D, L);
 }
 
 int rst_causal_conv1d_bwd(const void* x, int32_t dtype, const float* weight, const float* bias, const void* state_in,

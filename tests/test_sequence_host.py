@@ -281,3 +281,13 @@ def test_updates_move_the_version_counter(fake, monkeypatch):
     empty = fake(0, 6, 3)
     sequence.causal_conv1d_update(fake(0, 6), empty, fake(6, 4))
     assert empty._version == 0 and len(calls) == 8
+
+
+def test_workspace_sizes_of_shapes_out_of_range():
+    """0 bytes, as for an empty shape, and the reason: a row of 2^35 tokens used to end the process in a division by zero."""
+    lib = _lib.load()
+    for B, D, L in ((1, 1, 1 << 35), (1, 1, (1 << 31) + 1), (1 << 16, 1 << 15, 8), (-1, 4, 8), (4, 4, -8)):
+        assert lib.rst_causal_conv1d_bwd_workspace_bytes(B, D, L) == 0, (B, D, L)
+        assert b"causal_conv1d_bwd_workspace_bytes" in lib.rst_last_error()
+    assert lib.rst_causal_conv1d_bwd_workspace_bytes(1, 1, 1 << 31) > 0
+    assert lib.rst_causal_conv1d_bwd_workspace_bytes(1 << 15, 1 << 15, 8) > 0
