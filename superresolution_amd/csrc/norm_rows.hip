@@ -264,9 +264,16 @@ static NormRowsPlan norm_rows_plan(int C, int full_vec) {
     return p;
 }
 
-size_t norm_rows_bwd_ws_bytes(int64_t rows, int C) {
-    (void)rows;
-    return (size_t)NR_BWD_BLOCKS * 2 * (size_t)C * sizeof(float);
+// blocks of the backward kernel, each with a row of partial sums [2][C]
+static int64_t norm_rows_bwd_grid(int64_t rows, int lpr) {
+    const int64_t want = cdiv(rows, 256 / lpr);
+    return want < NR_BWD_BLOCKS ? want : NR_BWD_BLOCKS;
+}
+static size_t norm_rows_bwd_ws_bytes(int64_t rows, int C) {
+    // (of the two types' plans the one with more blocks: the size is asked for without a type)
+    const int64_t a = norm_rows_bwd_grid(rows, norm_rows_plan(C, Store<float>::VEC).lpr);
+    const int64_t b = norm_rows_bwd_grid(rows, norm_rows_plan(C, Store<bf16_t>::VEC).lpr);
+    return (size_t)(a > b ? a : b) * 2 * (size_t)C * sizeof(float);
 }
 
 // The pairs that the plan comes to for some length, fp32 (4 values a vector) or bf16 (8)
@@ -314,8 +321,7 @@ static int norm_rows_bwd_t(const T* x, const float* w, int with_bias, const T* d
                            int64_t rows, int C, float eps, float* partial, hipStream_t st) {
     constexpr int V = Store<T>::VEC;
     const NormRowsPlan p = norm_rows_plan(C, V);
-    const int64_t want = cdiv(rows, 256 / p.lpr);
-    const int grid = (int)(want < NR_BWD_BLOCKS ? want : NR_BWD_BLOCKS);
+    const int grid = (int)norm_rows_bwd_grid(rows, p.lpr);
     ProfScope prof(st, "rows_norm_bwd", 14.0 * rows * C, 3.0 * sizeof(T) * rows * C);
     NR_DISPATCH(norm_rows_bwd_kernel, (size_t)(256 / p.lpr) * C * sizeof(float), grid, x, w, with_bias, dy, dx, partial, rows, C, eps);
     hipLaunchKernelGGL(norm_rows_reduce_kernel, dim3((unsigned)cdiv(C, 16), with_bias ? 2 : 1), dim3(1024), 0, st, partial, grid, C,

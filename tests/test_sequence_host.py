@@ -291,3 +291,12 @@ def test_workspace_sizes_of_shapes_out_of_range():
         assert b"causal_conv1d_bwd_workspace_bytes" in lib.rst_last_error()
     assert lib.rst_causal_conv1d_bwd_workspace_bytes(1, 1, 1 << 31) > 0
     assert lib.rst_causal_conv1d_bwd_workspace_bytes(1 << 15, 1 << 15, 8) > 0
+
+
+def test_norm_workspace_fits_the_rows():
+    """A row of partial sums for every block that runs: at most 1024, and no more than there are rows."""
+    size = _lib.load().rst_rows_norm_bwd_workspace_bytes
+    assert size(1, 8192) == 8192 * 8 and size(64, 384) <= 64 * 384 * 8 and size(1 << 20, 96) == 1024 * 96 * 8
+    for C in (1, 5, 24, 96, 181, 513, 1000, 2048, 4096, 8192):
+        sizes = [size(rows, C) for rows in (1, 2, 7, 64, 1000, 1 << 20)]
+        assert sizes == sorted(sizes) and sizes[0] == 8 * C and sizes[-1] == 1024 * 8 * C, C
