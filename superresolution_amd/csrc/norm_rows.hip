@@ -16,7 +16,7 @@
 //
 // A row whose length is no multiple of the vector ends in a vector that is pulled back to the row's end: its first
 // values are the neighbour's last ones again, left out of every sum and stored twice with the same bits.
-// Forward 134 us for 1048576 x 96 fp32 (6.0 TB/s), 13.4 us for 131072 x 96 bf16 (3.8 TB/s: launch and fill count there),
+// Forward 134 us for 1048576 x 96 fp32 (6.0 TB/s), 12.1 us for 131072 x 96 bf16 (4.2 TB/s: launch and fill count there),
 // 3.6 us, a launch, for 64 x 384.
 #include "seq_common.hpp"
 
@@ -102,7 +102,7 @@ norm_rows_fwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
 }
 
 // Blocks walk over the rows, the next row's values on the way (448 -> 240 us for 1048576 x 96 fp32: 5.0 TB/s; 131072 x 96 bf16:
-// 20.5 us, 3.7 TB/s); a lane keeps the sums of dw and db of its own columns in registers, the block adds those of its row
+// 21.0 us, 3.6 TB/s); a lane keeps the sums of dw and db of its own columns in registers, the block adds those of its row
 // groups through LDS and writes one row of partial sums [2][C]; norm_rows_reduce_kernel adds the blocks' rows in a fixed order
 // (the same bits run to run; 4 to 5 us).
 template <typename T, int VEC, int LPR, int NV>
@@ -248,6 +248,11 @@ struct NormRowsPlan { int vec, lpr, nv; };
 // shorter butterfly) where two are alike.  Against one vector a lane, the next power of two of them, forward: 1048576 x 96
 // fp32 136 to 205 us, 262144 x 192 bf16 37 to 47, 262144 x 130 bf16 29 to 40, 262144 x 48 fp32 20.4 to 21.7.  A lane holds at
 // most 24 values of a bf16 row: 32 take all 256 registers.
+// Rows beyond 64 lanes (1536 values bf16, 1024 fp32) go to the 256 lanes of a block with 2, 4 or 8 vectors, where up to half of the
+// vectors are idle and the backward kernel spills with 4 fp32 vectors (26 registers).  For 2^28 values bf16 (2^27 fp32) the
+// forward kernel reaches 5.6 to 5.9 TB/s at 512 to 1536 values a row and the backward kernel 4.8 to 5.0; with 256 lanes bf16 rows of
+// 1600, 2048 and 4096 values come to 3.7, 4.4 and 4.9 forward and 1.9, 2.4 and 3.6 backward, fp32 rows of 2048, 2500, 4096 and 8192
+// to 5.8, 5.3, 5.4 and 5.5 forward and 5.0, 1.8, 2.4 and 4.1 backward.
 static NormRowsPlan norm_rows_plan(int C, int full_vec) {
     const int most = full_vec == 8 ? 3 : 4;
     NormRowsPlan p{full_vec, 0, 0};

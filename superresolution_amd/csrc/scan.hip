@@ -7,7 +7,7 @@
 //   dC_t[n] = sum_d h e,  dB_t[n] = sum_d g dt x,  dx = dt sum_n g B + D e,  ddt = x sum_n g B + sum_n A a g h_{t-1},
 //   dA[n] = sum_{b,t} dt a g h_{t-1},  dD = sum e x,  ddelta = ddt sigmoid(delta + bias),  dz = dy s silu'(z)
 //
-// Bound by the vector pipe, not by memory: one exponential and five more operations per state and token forward (16
+// Bound by the vector pipe and its waits, not by memory: one exponential and five more operations per state and token forward (16
 // states: 96 operations for the 6 to 12 bytes of a bf16 or fp32 token), so the layout serves the instruction stream:
 //   - a lane is a channel and holds four of its states; the waves of a block hold the other states of the same 64
 //     channels.  B and C are then the same for a whole wave: one register holds its share of a tile and is the broadcast
@@ -215,9 +215,11 @@ __device__ __forceinline__ float gate_of(const Quad<T>& z, int i) {
 }
 
 // ---- what a chunk adds to the state behind it (REV: to the state's gradient before it), and the sum of its dt -------
-// 8 x 384 x 16384 bf16 of 16 states: 167 us, REV with a gate 186 (4.8 and 4.3 T state updates a second).
+// 8 x 384 x 16384 bf16 of 16 states: 163 us, REV with a gate 180 (4.9 and 4.5 T state updates a second).  Its 18.5 and 20.5 vector
+// instructions a token and wave, softplus (and gate) among them, come to 98 and 108 us at the bare rates of eight waves; a wave issues 27 % of its
+// time, waits 46 % for its turn and 27 % at counters and the two barriers of a tile.
 template <typename T, int W, bool Z, bool REV>
-__global__ void __launch_bounds__(64 * W, 8)                               // (at most 256 registers: else the matrix results go to AGPRs and back)
+__global__ void __launch_bounds__(64 * W, 8)                               // (eight waves a SIMD: at most 64 registers, and the matrix results stay in them)
 scan_chunk_kernel(const Scan a) {
     constexpr int NI = ScanItems<W>::N;
     __shared__ float dts[ST][SROW], us[ST][SROW];
@@ -373,8 +375,10 @@ __device__ __forceinline__ float start_state(const Scan& a, const ScanPlace& p, 
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
-// 8 x 384 x 16384 bf16 of 16 states, gated, the states before every tile kept: 261 us (3.1 T state updates a second; 604 MB, 2.3
-// TB/s).  80 registers and 25.5 KiB: six blocks a compute unit.
+// 8 x 384 x 16384 bf16 of 16 states, gated, the states before every tile kept: 257 us (3.1 T state updates a second; 558 MB fetched and 332
+// written, 3.5 TB/s).  At most 80 registers and, with 16 states, 25.5 KiB: six blocks a compute unit.  Its 28 vector instructions a token and
+// wave, five of them exponentials and the like, come to 138 us at the bare rates of eight waves; a wave issues 24 % of its
+// time, waits 42 % for its turn and 37 % at LDS, counters and barriers.
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, 6)
 scan_fwd_kernel(const Scan a) {
@@ -711,8 +715,10 @@ __device__ __forceinline__ void scan_bwd_body(const Scan& a, const ScanPlace& p,
     }
 }
 
-// 8 x 384 x 16384 bf16 of 16 states, gated: 793 us (1.0 T state updates a second): the 256 registers that hold the tile's states and
-// decays leave two waves a SIMD, which keep the vector pipe busy 75 % of the time (forward: six, 82 %).
+// 8 x 384 x 16384 bf16 of 16 states, gated: 782 us (1.0 T state updates a second): the 256 registers that hold the tile's states and
+// decays leave two waves a SIMD.  85 vector instructions a token and wave come to 435 us at the bare rates of two waves; a
+// wave issues 47 % of its time, waits 16 % for its turn and 37 % at LDS, counters and barriers, which one other wave does not cover.
+// Both bodies in one kernel spill 32 registers with a gate and 16 states, nearly all before the loop.
 template <typename T, int W, bool Z>
 __global__ void __launch_bounds__(64 * W, W >= 4 ? 2 : 1)                  // (fewer waves have more tokens a lane: 256 registers would spill)
 scan_bwd_kernel(const Scan a) {
@@ -773,7 +779,7 @@ scan_reduce_kernel(const Scan a, int W, int bcs, float* __restrict__ dA, float* 
 }
 
 // ---- one token -----------------------------------------------------------------------------------------------------
-// NL lanes share a channel, four states each.  Bound by the state's 8 N bytes per channel (256 x 768 of 16 states: 9.5 us, 2.7
+// NL lanes share a channel, four states each.  Bound by the state's 8 N bytes per channel (256 x 768 of 16 states: 9.7 us, 2.6
 // TB/s; 1 x 384: 3.5 us, a launch).  state_out may be the state.
 template <typename T, int NL>
 __global__ void __launch_bounds__(256)
@@ -840,9 +846,13 @@ static int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8;
 // clock and compute unit with one, two, four and eight waves, so one alone takes 2.4 shares (backward 1.9) and k take about
 // k + 1/2 (backward k).  Chunks cost the pass over their own states, 0.6 of the forward kernel's time and 0.2 of the
 // backward's, a block about half a tile beside its tiles, and the chain about three.  The number that costs least is
-// taken, chunks of at least two tiles.  Measured, 8 x 384 x 16384 bf16: forward 784, 546, 463, 449, 440, 454 us with 5, 10, 16,
+// taken, chunks of at least two tiles.  Measured, 8 x 384 x 16384 bf16 of 16 states: forward 784, 546, 463, 449, 440, 454 us with 5, 10, 16,
 // 21, 32, 48 chunks, backward 1497, 1068, 1065, 1020, 1020, 1047; one 16384-token prompt of 192 channels 70, 61, 53, 46, 45, 46
 // us with 64, 85, 128, 171, 256, 512.
+// The figures are those of 16 states, blocks of four waves; the other forms are planned with them.  What is chosen against the best of
+// eleven counts, gated bf16, us: 4 x 384 x 4096 forward 61 / 59, 64 / 59, 74 / 64, 111 / 97 with 4, 8, 16, 32 states, backward 174 / 118
+// (one-wave blocks: four fit a compute unit), 147 / 145, 151 / 151, 267 / 259; 8 x 384 x 16384 forward 328 / 319, 351 / 345, 369 / 367,
+// 614 / 614, backward 760 / 704, 863 / 861, 917 / 916, 1793 / 1793.
 static void scan_plan(Scan* a, bool bwd) {
     a->Dg = a->D / a->G;
     a->cb = (int)cdiv(a->Dg, SC);

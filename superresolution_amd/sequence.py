@@ -373,8 +373,9 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     `x`, `delta`, `z`: (batch, channel, token).  `A`: (channel, state), up to 32 states.  `B`, `C`: (batch, group, state,
     token), channel d reads group ``d // (channels / groups)`` -- or (batch, state, token) for one group.  `D`,
     `delta_bias`: (channel).  `initial_state` and, with `return_last_state`, the second result: (batch, channel, state),
-    fp32.  At most 2^24 tokens a call.  A token leaves the state alone where its step size is zero (`delta` = -inf under the softplus, and a finite
-    `x`): that is how sequences of different lengths are padded.  Differentiable in every tensor; for that the states
+    fp32.  At most 2^24 tokens a call.  A token leaves the state alone where its step size is zero (`delta` = -inf under the softplus, and finite
+    values in the other tensors, `dy` included): that is how sequences of different lengths are padded.  A rate in `A` may be
+    -inf, a state that every token with a step size above 1e-28 forgets.  batch x groups: at most 65535.  Differentiable in every tensor; for that the states
     of every 16th token are kept.  Counterpart in the reference: the scan that model/basicsr/archs/mambairv2_arch.py:384-390
     calls, with the same order of its first six arguments."""
     if x.dim() != 3:
