@@ -13,6 +13,7 @@
 // The mean is summed relative to the row's first value: of a flat row every difference is an exact zero, so its mean is its
 // value and its variance zero.  (The sum of the values themselves is a rounded one: 96 values of 1000.1 fp32 came to a mean
 // 6e-5 off, which 1 / sqrt(eps) makes 0.02 of.)  A row's own spread bounds the differences' roundings in any case.
+// Half the differences, each over C, are added up, so that no row of finite values overflows here.
 //
 // A row whose length is no multiple of the vector ends in a vector that is pulled back to the row's end: its first
 // values are the neighbour's last ones again, left out of every sum and stored twice with the same bits.
@@ -63,13 +64,12 @@ norm_rows_fwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
         row_vec<VEC>(lane + j * LPR, C, &start[j], &dup[j]);
         raw[j].load(xr + start[j]);
     }
-    const float first = Store<T>::get(xr[0]);
+    const float first = Store<T>::get(xr[0]), invC = 1.0f / (float)C;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s += i >= dup[j] ? raw[j].get(i) - first : 0.f;
-    const float invC = 1.0f / (float)C;
-    const float mu = fmaf(row_sum<LPR>(s, red), invC, first);
+        for (int i = 0; i < VEC; ++i) s = fmaf(i >= dup[j] ? fmaf(0.5f, raw[j].get(i), -0.5f * first) : 0.f, invC, s);
+    const float mu = fmaf(2.0f, row_sum<LPR>(s, red), first);
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -148,8 +148,8 @@ norm_rows_bwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s += i >= dup[j] ? rx[j].get(i) - first : 0.f;
-        const float mu = fmaf(row_sum<LPR>(s, red), invC, first);
+            for (int i = 0; i < VEC; ++i) s = fmaf(i >= dup[j] ? fmaf(0.5f, rx[j].get(i), -0.5f * first) : 0.f, invC, s);
+        const float mu = fmaf(2.0f, row_sum<LPR>(s, red), first);
         float q = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)

@@ -169,7 +169,8 @@ class _LayerNormFn(torch.autograd.Function):
 def layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension of `x` (..., C), C <= 8192: ``(x - mean) / sqrt(var + eps) * weight + bias``, or
     without a `bias` the bias-free norm ``x / sqrt(var + eps) * weight`` (the variance is still the centred one), as
-    ``WithBias_LayerNorm`` and ``BiasFree_LayerNorm`` (reference: model/Restromer.py:28-61).  `ops.layernorm` is the
+    ``WithBias_LayerNorm`` and ``BiasFree_LayerNorm`` (reference: model/Restromer.py:28-61).  The variance is fp32: rows that
+    spread by more than 1e19 are out of range.  `ops.layernorm` is the
     same norm over the channels of an NCHW image."""
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_WIDTH:
         raise RuntimeError(f"layernorm: x {tuple(x.shape)} (the last dimension: 1 to {MAX_NORM_WIDTH})")

@@ -880,3 +880,16 @@ def test_selective_scan_more_tokens_than_one_row_of_blocks():
         assert err <= 2 * n * 2.0 ** -24 + 2 * 2.0 ** -8, (name, err)
     for at in (0, 1, 31, 62, 63):
         assert not whole[2][at, ..., :-K].any() and not whole[3][at, ..., :-K].any() and not whole[0][at, ..., :-K].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [6, 96, 400, 1030])
+def test_layernorm_rows_with_the_lowest_value(C, dtype):
+    """A row of the type's lowest value is flat, though its sum does not fit fp32.  A row that starts with one and is zero behind
+    it has a variance that does not fit: its root is infinite and the norm the bias, as without the sum's detour over the
+    first value."""
+    x = torch.full((2, C), torch.finfo(dtype).min, dtype=dtype)
+    x[1, 1:] = 0.0
+    b = _rand(_gen(C), C)
+    y = sequence.layernorm(x.cuda(), torch.ones(C, device="cuda"), b.cuda())
+    assert torch.equal(y, b.cuda().to(dtype).expand(2, C))
