@@ -66,7 +66,7 @@ def test_lane_exchanges_wait(src, tmp_path):
     assert not found, found[:5]
 
 
-def test_checker_counts_wait_states():
+def test_counting_of_wait_states():
     early = "\tv_cvt_pk_bf16_f32 v1, v2, v3\n\ts_nop 0\n\tv_permlane16_swap_b32_e32 v0, v1\n"
     late = early.replace("s_nop 0", "s_nop 1")
     dpp = "\tv_add_f32_e32 v1, v2, v3\n\tv_mov_b32_dpp v4, v1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
