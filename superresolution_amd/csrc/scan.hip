@@ -375,8 +375,8 @@ __device__ __forceinline__ float start_state(const Scan& a, const ScanPlace& p, 
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
-// 8 x 384 x 16384 bf16 of 16 states, gated, the states before every tile kept: 257 us (3.1 T state updates a second; 558 MB fetched and 332
-// written, 3.5 TB/s).  At most 80 registers and, with 16 states, 25.5 KiB: six blocks a compute unit.  Its 28 vector instructions a token and
+// 8 x 384 x 16384 bf16 of 16 states, gated, the states before every tile kept: 257 us (3.1 T state updates a second; 604 MB, 2.3
+// TB/s).  At most 80 registers and, with 16 states, 25.5 KiB: six blocks a compute unit.  Its 28 vector instructions a token and
 // wave, five of them exponentials and the like, come to 138 us at the bare rates of eight waves; a wave issues 24 % of its
 // time, waits 42 % for its turn and 37 % at LDS, counters and barriers.
 template <typename T, int W, bool Z>
