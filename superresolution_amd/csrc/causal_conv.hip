@@ -10,7 +10,7 @@
 // lanes along a short one (so that a wave has 8 rows); a row of fewer than 8 tokens is one lane's.
 // A row whose length is no multiple of 8 ends in a chunk that is pulled back to the row's end: its first tokens are
 // stored twice with the same bits and left out of the weight's sums.
-// 8 x 384 x 4096 bf16: 12.0 us forward (4.2 TB/s), 21.4 backward (3.5 TB/s, below the 4.8 of a copy: two loads more a tensor for the
+// 8 x 384 x 4096 bf16: 12 to 13 us forward (3.9 to 4.2 TB/s), 21 to 22 backward (3.5 TB/s, below the 4.8 of a copy: two loads more a tensor for the
 // neighbours' tokens) and 3.9 for the sums of the weight's shares; a token, or a piece of a thousand, is a launch: 2 to 4 us.
 #include "seq_common.hpp"
 

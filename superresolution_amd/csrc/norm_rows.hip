@@ -17,7 +17,7 @@
 //
 // A row whose length is no multiple of the vector ends in a vector that is pulled back to the row's end: its first
 // values are the neighbour's last ones again, left out of every sum and stored twice with the same bits.
-// Forward 134 us for 1048576 x 96 fp32 (6.0 TB/s), 12.1 us for 131072 x 96 bf16 (4.2 TB/s: launch and fill count there),
+// Forward 134 us for 1048576 x 96 fp32 (6.0 TB/s), 12 to 14 us for 131072 x 96 bf16 (3.6 to 4.2 TB/s: launch and fill count there),
 // 3.6 us, a launch, for 64 x 384.
 #include "seq_common.hpp"
 
@@ -102,7 +102,7 @@ norm_rows_fwd_kernel(const T* __restrict__ x, const float* __restrict__ weight, 
 }
 
 // Blocks walk over the rows, the next row's values on the way (448 -> 240 us for 1048576 x 96 fp32: 5.0 TB/s; 131072 x 96 bf16:
-// 21.0 us, 3.6 TB/s); a lane keeps the sums of dw and db of its own columns in registers, the block adds those of its row
+// 21 us, 3.6 TB/s); a lane keeps the sums of dw and db of its own columns in registers, the block adds those of its row
 // groups through LDS and writes one row of partial sums [2][C]; norm_rows_reduce_kernel adds the blocks' rows in a fixed order
 // (the same bits run to run; 4 to 5 us).
 template <typename T, int VEC, int LPR, int NV>
